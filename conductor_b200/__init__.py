@@ -10,10 +10,11 @@ from ``libconductor_b200.so`` reached through a C ABI.
 """
 __version__ = "0.1.0"
 
+from . import ops
 from .compiler.gcu_backend import GCUBackend, get_gcu_backend, register_gcu_backend
 from .utils.config import get_config
 
-__all__ = ["register_gcu_backend", "GCUBackend", "get_gcu_backend", "get_config"]
+__all__ = ["register_gcu_backend", "GCUBackend", "get_gcu_backend", "get_config", "ops"]
 
 try:
     register_gcu_backend()

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from dataclasses import dataclass, field
 from typing import Any, Optional
 
@@ -70,6 +71,14 @@ class CdrAttnParams(ctypes.Structure):
     _fields_ = [("scale", ctypes.c_float), ("causal", ctypes.c_int32)]
 
 
+class CdrWindowAttnParams(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("has_lengths", ctypes.c_int32), ("window", ctypes.c_int64), ("sinks", ctypes.c_int64)]
+
+
+class CdrPrefixAttnParams(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("has_lengths", ctypes.c_int32)]
+
+
 class CdrLaunchItem(ctypes.Structure):
     """``cdr_launch_item``: the arguments of one ``cdr_launch`` call, for ``cdr_launch_many``."""
 
@@ -94,18 +103,24 @@ class KernelLaunch:
     alias_of: Optional[Buffer] = None   # SHAPE clusters: output is a view of this buffer
     cluster: Optional[FusionCluster] = None
     needs_workspace: bool = False
+    # scratch comes from torch's caching allocator at every call (inside a capture: from the graph's own
+    # pool) instead of being kept per launch: calls of one launch on several streams, and two captured
+    # graphs of it, never share it
+    per_call_workspace: bool = False
     view_strides: Optional[tuple] = None  # COPY launches: element strides of the view of inputs[0] that is gathered
     view_offset: int = 0                  # COPY launches: first element of that view, relative to inputs[0]'s own
     out_view: Optional[tuple] = None      # COPY launches that fill one part of outputs[0] (cat): (shape, strides, offset)
     # the executor's marshalled form of this launch (shape signature, descriptor arrays, parameter pointer):
     # built on first use, reused while shapes, strides and dtypes stay the same
     _marshal: Any = field(default=None, repr=False, compare=False)
+    _workspace_size: Any = field(default=None, repr=False, compare=False)   # (signature, bytes) with per_call_workspace
 
     def describe(self) -> str:
         ins = ", ".join(b.name for b in self.inputs)
         outs = ", ".join(f"{b.name}:{b.scope.value}" for b in self.outputs)
         tname = {0: "alias", 1: "elementwise", 2: "row_reduce", 3: "softmax_fwd", 4: "softmax_bwd",
-                 5: "gemm_epilogue", 6: "attention", 7: "full_reduce", 8: "layer_norm", 9: "copy", 10: "col_sum"}[self.template]
+                 5: "gemm_epilogue", 6: "attention", 7: "full_reduce", 8: "layer_norm", 9: "copy", 10: "col_sum",
+                 11: "window_attention", 12: "prefix_attention"}[self.template]
         return f"{outs} = {tname}<{self.name}>({ins})"
 
 
@@ -608,6 +623,8 @@ def _lower_gemm(cluster: FusionCluster) -> KernelLaunch:
 
 
 def _lower_attention(cluster: FusionCluster) -> KernelLaunch:
+    if cluster.nodes[0].op_name in ("window_attention", "prefix_attention"):
+        return _lower_cache_attention(cluster)
     _require_shapes(cluster)
     node = cluster.nodes[0]
     kw = node.metadata.get("kwargs", {})
@@ -633,6 +650,61 @@ def _lower_attention(cluster: FusionCluster) -> KernelLaunch:
     p = CdrAttnParams(float(scale), 1 if causal else 0)
     return KernelLaunch(Template.ATTENTION, cluster.signature(), bufs, [out], p, [out.shape], [out.dtype],
                         cluster=cluster, needs_workspace=True)
+
+
+def _attention_scale(scale, head_dim) -> float:
+    return 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+
+
+def window_attention_launch(name, q_shape, dtype, window, sinks, has_lengths, scale, cluster=None, inputs=(), outputs=()) -> KernelLaunch:
+    """One launch of the window-attention template (inputs: q, k, v[, lengths])."""
+    _require_head_dim("window_attention", q_shape)
+    window, sinks = operator.index(window), operator.index(sinks)
+    if window < 1 or sinks < 0:
+        raise UnsupportedOperationError("window_attention", f"window={window}, sinks={sinks}: window must be at least 1 and sinks at least 0")
+    most = 2 ** 62                                             # the parameter block holds 64-bit integers
+    p = CdrWindowAttnParams(_attention_scale(scale, q_shape[-1]), 1 if has_lengths else 0, min(window, most), min(sinks, most))
+    return KernelLaunch(Template.WINDOW_ATTENTION, name, list(inputs), list(outputs), p, [tuple(q_shape)], [dtype], cluster=cluster,
+                        needs_workspace=True, per_call_workspace=True)
+
+
+def prefix_attention_launch(name, q_shape, dtype, has_lengths, scale, cluster=None, inputs=(), outputs=()) -> KernelLaunch:
+    """One launch of the prefix-attention template (inputs: q, prefix_k, prefix_v, k, v[, lengths])."""
+    _require_head_dim("prefix_attention", q_shape)
+    p = CdrPrefixAttnParams(_attention_scale(scale, q_shape[-1]), 1 if has_lengths else 0)
+    return KernelLaunch(Template.PREFIX_ATTENTION, name, list(inputs), list(outputs), p, [tuple(q_shape)], [dtype], cluster=cluster,
+                        needs_workspace=True, per_call_workspace=True)
+
+
+def _require_head_dim(name, q_shape) -> None:
+    if len(q_shape) != 4 or q_shape[-1] not in (64, 128):
+        raise UnsupportedOperationError(name, f"q of shape {tuple(q_shape)}: expected [batch, heads, queries, 64 or 128]")
+
+
+def _lower_cache_attention(cluster: FusionCluster) -> KernelLaunch:
+    """window_attention(q, k, v, window, sinks, lengths, scale) and
+    prefix_attention(q, prefix_k, prefix_v, k, v, lengths, scale) of ``conductor_b200/ops.py``."""
+    _require_shapes(cluster)
+    node = cluster.nodes[0]
+    names = (["q", "k", "v", "window", "sinks", "lengths", "scale"] if node.op_name == "window_attention"
+             else ["q", "prefix_k", "prefix_v", "k", "v", "lengths", "scale"])
+    args = dict(zip(names, node.metadata.get("arg_spec", [])), **node.metadata.get("kwarg_spec", {}))
+    bufs = []
+    for name in names:
+        kind, val = args.get(name, ("const", None))
+        if kind == "buf":
+            if name in ("window", "sinks", "scale"):
+                raise UnsupportedOperationError(node.op_name, f"{name} must be a Python number")
+            bufs.append(node.inputs[val])
+        elif name not in ("window", "sinks", "scale") and not (name == "lengths" and val is None):
+            raise UnsupportedOperationError(node.op_name, f"{name} must be a tensor")
+    out = node.outputs[0]
+    has_lengths = args.get("lengths", ("const", None))[0] == "buf"
+    scale = args.get("scale", ("const", None))[1]
+    if node.op_name == "prefix_attention":
+        return prefix_attention_launch(cluster.signature(), out.shape, out.dtype, has_lengths, scale, cluster, bufs, [out])
+    return window_attention_launch(cluster.signature(), out.shape, out.dtype, args["window"][1], args.get("sinks", ("const", 0))[1],
+                                   has_lengths, scale, cluster, bufs, [out])
 
 
 def _lower_cat(cluster: FusionCluster) -> list:

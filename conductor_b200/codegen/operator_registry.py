@@ -52,6 +52,7 @@ class Template:
     """cdr_template ids."""
 
     ELEMENTWISE, ROW_REDUCE, SOFTMAX_FWD, SOFTMAX_BWD, GEMM_EPILOGUE, ATTENTION, FULL_REDUCE, LAYER_NORM, COPY, COL_SUM = range(1, 11)
+    WINDOW_ATTENTION, PREFIX_ATTENTION = 11, 12
 
 
 @dataclass(frozen=True)
@@ -161,6 +162,11 @@ class OperatorRegistry:
                        preferred_fusion_level=FusionLevel.GLOBAL))
         r(OperatorInfo("scaled_dot_product_attention", "attention", OpType.ATTENTION, False, 3,
                        template=Template.ATTENTION, preferred_fusion_level=FusionLevel.GLOBAL), "attention")
+        # attention over a key/value cache (conductor_b200/ops.py)
+        r(OperatorInfo("window_attention", "window_attention", OpType.ATTENTION, False, 3,
+                       template=Template.WINDOW_ATTENTION, preferred_fusion_level=FusionLevel.GLOBAL))
+        r(OperatorInfo("prefix_attention", "prefix_attention", OpType.ATTENTION, False, 5,
+                       template=Template.PREFIX_ATTENTION, preferred_fusion_level=FusionLevel.GLOBAL))
         # metadata-only reshapes of contiguous tensors: no kernel
         # layout changes that move data: one launch of the strided-copy template
         for perm_op in ("transpose", "permute", "t", "swapaxes", "movedim"):

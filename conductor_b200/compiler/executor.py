@@ -44,6 +44,21 @@ def make_descriptors(tensors: Sequence[torch.Tensor]):
     return arr
 
 
+# Templates that read their operands' strides: a view is passed as it is when the kernel can address it.
+_STRIDED_ATTENTION = (Template.WINDOW_ATTENTION, Template.PREFIX_ATTENTION)
+
+
+def _attention_view_ok(t: torch.Tensor) -> bool:
+    """A view the cache-attention templates read in place: contiguous last dimension, 16-byte aligned
+    start, every other stride a positive multiple of 16 bytes (lengths: contiguous)."""
+    if t.is_contiguous():
+        return t.dim() < 3 or t.data_ptr() % 16 == 0
+    if t.dim() < 3:
+        return False
+    *outer, last = zip(t.shape, t.stride())
+    return last[1] == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or (st > 0 and st % 8 == 0) for n, st in outer)
+
+
 def raise_for_status(lib, status: int, name: str) -> None:
     if status == 0:
         return
@@ -102,6 +117,20 @@ class GCUKernelExecutor:
         self._workspaces[key] = (sig, ws)
         return ws
 
+    def fresh_workspace(self, launch: KernelLaunch, ins, outs, in_desc, out_desc, params_ptr, params_size):
+        """Scratch of this call alone, from torch's caching allocator: it returns to the pool of the current
+        stream as soon as the launch is enqueued.  Only its size is kept, per shape signature."""
+        sig = launch._marshal[0]
+        if launch._workspace_size is None or launch._workspace_size[0] is not sig:
+            need = ctypes.c_size_t(0)
+            with torch.cuda.device(ins[0].device):
+                rc = self.lib.cdr_workspace_bytes(launch.template, in_desc, len(ins), out_desc, len(outs), params_ptr,
+                                                  params_size, ctypes.byref(need))
+            raise_for_status(self.lib, rc, launch.name)
+            launch._workspace_size = (sig, need.value)
+        n = launch._workspace_size[1]
+        return torch.empty(n, dtype=torch.uint8, device=ins[0].device) if n else None
+
     def _prepare(self, launch: KernelLaunch, inputs: Sequence[torch.Tensor], outputs):
         """Marshal one launch: contiguous inputs, allocated outputs, descriptor arrays (built once
         per launch and shape signature, data pointers refreshed per call), parameter block, scratch."""
@@ -112,6 +141,10 @@ class GCUKernelExecutor:
             raise DeviceError(f"kernel templates run on CUDA tensors, got {device}")
         if launch.template == Template.COPY:
             ins = list(inputs)                      # the view's strides are the point
+        elif launch.template in _STRIDED_ATTENTION:
+            if any(t.device != device for t in inputs):
+                raise DeviceError(f"{launch.name}: inputs on different devices")
+            ins = [t if _attention_view_ok(t) else self.make_contiguous(t) for t in inputs]
         else:
             ins = [t if t.is_contiguous() else self.make_contiguous(t) for t in inputs]
         if outputs is None:
@@ -135,7 +168,9 @@ class GCUKernelExecutor:
             for i, t in enumerate(outputs):
                 out_desc[i].data = t.data_ptr()
         ws = None
-        if launch.needs_workspace:
+        if launch.per_call_workspace:
+            ws = self.fresh_workspace(launch, ins, outputs, in_desc, out_desc, params_ptr, params_size)
+        elif launch.needs_workspace:
             ws = self.workspace_for(launch, ins, outputs, in_desc, out_desc, params_ptr, params_size)
         return device, ins, outputs, in_desc, out_desc, params_ptr, params_size, ws
 

@@ -58,6 +58,13 @@ def batch_inputs(dag) -> tuple[int, list[int]]:
                 ok &= pos == 0
             elif node.op_name == "scaled_dot_product_attention":
                 ok &= pos < 3
+            elif node.op_name == "window_attention":
+                pass                              # q, k, v and the lengths all have one entry per sequence
+            elif node.op_name == "prefix_attention":
+                # so have q, k, v and the lengths, but not the prefix (arguments 1 and 2)
+                spec, kw = node.metadata.get("arg_spec", []), node.metadata.get("kwarg_spec", {})
+                shared = [s for s in list(spec[1:3]) + [kw.get("prefix_k"), kw.get("prefix_v")] if s is not None]
+                ok &= ("buf", pos) not in shared
             elif node.is_reduction():
                 ok &= pos == 0 and len(buf.shape) >= 2
             else:

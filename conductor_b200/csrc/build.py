@@ -31,6 +31,7 @@ SOURCES = {
     "cdr_copy.cu": [],
     "cdr_gemm.cu": [],
     "cdr_attention.cu": [],
+    "cdr_cache_attention.cu": [],
 }
 
 COMMON = [

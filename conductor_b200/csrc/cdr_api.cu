@@ -112,6 +112,8 @@ int check_params(int template_id, const void* params, size_t bytes) {
     case CDR_T_GEMM_EPILOGUE: want = sizeof(cdr_gemm_params); break;
     case CDR_T_ATTENTION: want = sizeof(cdr_attn_params); break;
     case CDR_T_LAYER_NORM: want = sizeof(cdr_norm_params); break;
+    case CDR_T_WINDOW_ATTENTION: want = sizeof(cdr_window_attn_params); break;
+    case CDR_T_PREFIX_ATTENTION: want = sizeof(cdr_prefix_attn_params); break;
     default:
       set_error("unknown template id %d", template_id);
       return CDR_ERR_UNSUPPORTED;
@@ -238,6 +240,10 @@ int cdr_workspace_bytes(int template_id, const cdr_tensor* inputs, int n_inputs,
     case CDR_T_FULL_REDUCE: return full_reduce_workspace(inputs, n_inputs, bytes_out);
     case CDR_T_ATTENTION: return attention_workspace(inputs, n_inputs, bytes_out);
     case CDR_T_COL_SUM: return col_sum_workspace(inputs, n_inputs, outputs, n_outputs, bytes_out);
+    case CDR_T_WINDOW_ATTENTION:
+      return window_attention_workspace(inputs, n_inputs, outputs, n_outputs, static_cast<const cdr_window_attn_params*>(params), bytes_out);
+    case CDR_T_PREFIX_ATTENTION:
+      return prefix_attention_workspace(inputs, n_inputs, outputs, n_outputs, static_cast<const cdr_prefix_attn_params*>(params), bytes_out);
     default: return CDR_OK;
   }
 }
@@ -263,6 +269,12 @@ int cdr_launch(int template_id, const cdr_tensor* inputs, int n_inputs, const cd
     case CDR_T_ATTENTION:
       return launch_attention(inputs, n_inputs, outputs, n_outputs, static_cast<const cdr_attn_params*>(params),
                               workspace, workspace_bytes, s);
+    case CDR_T_WINDOW_ATTENTION:
+      return launch_window_attention(inputs, n_inputs, outputs, n_outputs, static_cast<const cdr_window_attn_params*>(params),
+                                     workspace, workspace_bytes, s);
+    case CDR_T_PREFIX_ATTENTION:
+      return launch_prefix_attention(inputs, n_inputs, outputs, n_outputs, static_cast<const cdr_prefix_attn_params*>(params),
+                                     workspace, workspace_bytes, s);
     case CDR_T_COPY: return launch_strided_copy(inputs, n_inputs, outputs, n_outputs, s);
     case CDR_T_COL_SUM: return launch_col_sum(inputs, n_inputs, outputs, n_outputs, workspace, workspace_bytes, s);
     case CDR_T_LAYER_NORM:

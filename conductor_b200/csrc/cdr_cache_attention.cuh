@@ -1,0 +1,59 @@
+// The two attentions over a key/value cache (window_attention, prefix_attention), seen by their
+// kernels as one problem:
+//
+//   query row i of sequence b stands at position p = L_b - Sq + i of the sequence's own keys, where
+//   L_b = clamp(lengths[b], 0, Skv).  It sees
+//     - every key of the shared prefix (P keys per key head, P = 0 without one) and
+//     - own key j when  j <= p  and  (j > p - window  or  j < sinks).
+//   A row with p < 0 (a batch padded to Sq queries) sees nothing and its output is 0.
+//
+// Heads are grouped: query heads h*G .. h*G + G-1 share key head h.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cdr_common.cuh"
+
+namespace cdr {
+
+// element strides of one [B, H, S, D] operand (D contiguous)
+struct HeadStrides {
+  int64_t b, h, s;
+};
+
+struct CacheAttn {
+  const void *q, *k, *v, *pk, *pv;
+  void* out;
+  const void* lengths;  // [B] i32 / i64, or nullptr: every sequence uses all Skv keys
+  int lengths_i64;
+  HeadStrides sq, sk, sv, spk, spv, so;
+  int B, Hq, Hkv, G, Sq, Skv, P, D;
+  int window, sinks;    // clamped to 2^30: positions are below that
+  float scale_log2;     // scale * log2(e)
+  int bf16;
+};
+
+// Partial results of the shared prefix, one per key split and packed query row, in caller scratch:
+// O already divided by its sum, and log2 of the sum of exponentials (base 2, scaled scores).
+struct PrefixPartials {
+  const float* o;    // [splits][Hkv][rows][D]
+  const float* lse;  // [splits][Hkv][rows]
+  int splits;        // 0: none
+  int rows;          // B * Sq * G, row (b, i, g) at (b * Sq + i) * G + g
+};
+
+// Few query rows per key head: the keys are streamed once through registers (cdr_cache_attention.cu).
+// part.splits > 0: joined with the partial results; else the prefix is streamed as well.
+int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int sequence_length(const CacheAttn& a, int b) {
+  if (!a.lengths) return a.Skv;
+  const int64_t n = a.lengths_i64 ? __ldg(static_cast<const long long*>(a.lengths) + b)
+                                  : static_cast<int64_t>(__ldg(static_cast<const int*>(a.lengths) + b));
+  return n < 0 ? 0 : n > a.Skv ? a.Skv : static_cast<int>(n);
+}
+#endif
+
+}  // namespace cdr

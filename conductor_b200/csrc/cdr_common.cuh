@@ -90,6 +90,14 @@ int launch_layer_norm(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, i
 int launch_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,
                      const cdr_attn_params* p, void* ws, size_t ws_bytes, cudaStream_t stream);
 int attention_workspace(const cdr_tensor* ins, int n_in, size_t* bytes);
+int window_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,
+                               const cdr_window_attn_params* p, size_t* bytes);
+int launch_window_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,
+                            const cdr_window_attn_params* p, void* ws, size_t ws_bytes, cudaStream_t stream);
+int prefix_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,
+                               const cdr_prefix_attn_params* p, size_t* bytes);
+int launch_prefix_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,
+                            const cdr_prefix_attn_params* p, void* ws, size_t ws_bytes, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // ---- 128-bit streaming global access -------------------------------------

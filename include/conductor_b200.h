@@ -98,10 +98,16 @@ enum cdr_template {
                              broadcasts) into an output of the same shape: transpose / permute / slice /
                              expand / contiguous().  The output's strides are honoured too (positive,
                              non-overlapping), which writes one part of a concatenation; no params */
-  CDR_T_COL_SUM = 10      /* out[n] = sum over m of x[m, n] for a contiguous x viewed as [M, N] (N = the
+  CDR_T_COL_SUM = 10,     /* out[n] = sum over m of x[m, n] for a contiguous x viewed as [M, N] (N = the
                              output's element count): the bias gradient of a linear layer, `sum(dim=0)`.
                              fp32 accumulation in a fixed order (deterministic); no params; needs workspace.
                              The reference has no counterpart: it compiles no backward graphs */
+  CDR_T_WINDOW_ATTENTION = 11, /* causal attention over a key/value cache with a sliding window and
+                             always-visible first keys, inputs (q, k, v[, lengths]),
+                             params = cdr_window_attn_params; needs workspace                */
+  CDR_T_PREFIX_ATTENTION = 12  /* causal attention of a batch whose sequences share a prefix, inputs
+                             (q, prefix_k, prefix_v, k, v[, lengths]), params = cdr_prefix_attn_params;
+                             needs workspace                                                 */
 };
 
 /* ---- elementwise programs -------------------------------------------------
@@ -222,6 +228,29 @@ typedef struct cdr_attn_params {
   float scale;    /* softmax scale, e.g. 1/sqrt(head_dim) */
   int32_t causal; /* 1: key j attends only when j <= i    */
 } cdr_attn_params;
+
+/* Attention over a key/value cache (no counterpart in the reference, whose attention kernels take q, k and v of
+ * one length).  q is [B, Hq, Sq, D], k and v are [B, Hkv, Skv, D] with Hq a multiple of Hkv (query heads
+ * h*G .. h*G + G-1 share key head h), the output is shaped like q; bf16 / f16, D = 64 or 128.  D must be contiguous;
+ * the other strides are honoured (positive multiples of 8 elements), pointers 16-byte aligned.  The optional last input
+ * `lengths` ([B], i32 or i64, device memory like every input) is the number of keys each sequence uses,
+ * L = clamp(lengths[b], 0, Skv) (Skv without it); k and v behind L are never used, whatever they hold.  Query i stands at
+ * position p = L - Sq + i and sees key j when j <= p and (window attention) j > p - window or j < sinks.  A query with
+ * p < 0 (a padded batch) sees nothing, and a query that sees nothing has output 0.  Non-finite values in the used
+ * part of v may reach every query of the same head whose tile reads that key. */
+typedef struct cdr_window_attn_params {
+  float scale;         /* softmax scale, positive and finite             */
+  int32_t has_lengths; /* 1: lengths is the last input                   */
+  int64_t window;      /* >= 1; keys p - window + 1 .. p are visible     */
+  int64_t sinks;       /* >= 0; so are keys 0 .. sinks - 1 (where j <= p) */
+} cdr_window_attn_params;
+
+/* As above without a window: query i sees its sequence's keys j <= p and, when p >= 0, all P keys of the prefix
+ * (prefix_k, prefix_v: [Hkv, P, D], P >= 0), which every sequence of the batch has in front of its own. */
+typedef struct cdr_prefix_attn_params {
+  float scale;
+  int32_t has_lengths;
+} cdr_prefix_attn_params;
 
 /* ---- entry points --------------------------------------------------------- */
 
