@@ -32,6 +32,7 @@ SOURCES = {
     "cdr_gemm.cu": [],
     "cdr_attention.cu": [],
     "cdr_cache_attention.cu": [],
+    "cdr_tile_attention.cu": [],
 }
 
 COMMON = [

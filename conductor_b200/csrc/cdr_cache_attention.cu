@@ -548,8 +548,37 @@ int parse_prefix(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_
   return CDR_OK;
 }
 
-int run_cache_attention(const CacheAttn& a, void* ws, size_t ws_bytes, cudaStream_t stream) {
-  return launch_stream_attention(a, PrefixPartials{nullptr, nullptr, 0, 0}, stream);
+// Which kernels a call runs.
+enum class Path { kStream, kTile, kPacked };
+
+Path choose_path(const CacheAttn& a) {
+  if (a.Sq >= 64) return Path::kTile;
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
+  if (a.P >= 128 && rows <= 128 && a.B * rows > 32) return Path::kPacked;
+  return Path::kStream;
+}
+
+size_t cache_attention_workspace(const CacheAttn& a) {
+  switch (choose_path(a)) {
+    case Path::kTile: return kTileCounterBytes;
+    case Path::kPacked: return packed_workspace(a);
+    default: return 0;
+  }
+}
+
+int run_cache_attention(const CacheAttn& a, const char* op, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  const Path path = choose_path(a);
+  const size_t need = cache_attention_workspace(a);
+  if (need && (!ws || ws_bytes < need)) {
+    set_error("%s: workspace of %zu bytes required, got %zu", op, need, ws ? ws_bytes : (size_t)0);
+    return CDR_ERR_WORKSPACE;
+  }
+  if (need && !aligned16(ws)) { set_error("%s: workspace must be 16-byte aligned", op); return CDR_ERR_MISALIGNED; }
+  PrefixPartials part{nullptr, nullptr, 0, 0};
+  if (path == Path::kTile) return launch_tile_attention(a, ws, stream);
+  if (path == Path::kPacked)
+    if (int rc = launch_packed_prefix(a, ws, &part, stream)) return rc;
+  return launch_stream_attention(a, part, stream);
 }
 
 }  // namespace
@@ -559,7 +588,9 @@ int window_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor
   CacheAttn a;
   bool empty = false;
   *bytes = 0;
-  return parse_window(ins, n_in, outs, n_out, p, &a, &empty);
+  if (int rc = parse_window(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
+  if (!empty) *bytes = cache_attention_workspace(a);
+  return CDR_OK;
 }
 
 int prefix_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out, const cdr_prefix_attn_params* p,
@@ -567,7 +598,9 @@ int prefix_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor
   CacheAttn a;
   bool empty = false;
   *bytes = 0;
-  return parse_prefix(ins, n_in, outs, n_out, p, &a, &empty);
+  if (int rc = parse_prefix(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
+  if (!empty) *bytes = cache_attention_workspace(a);
+  return CDR_OK;
 }
 
 int launch_window_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out, const cdr_window_attn_params* p,
@@ -575,7 +608,7 @@ int launch_window_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* o
   CacheAttn a;
   bool empty = false;
   if (int rc = parse_window(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
-  return empty ? CDR_OK : run_cache_attention(a, ws, ws_bytes, stream);
+  return empty ? CDR_OK : run_cache_attention(a, "window_attention", ws, ws_bytes, stream);
 }
 
 int launch_prefix_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out, const cdr_prefix_attn_params* p,
@@ -583,7 +616,7 @@ int launch_prefix_attention(const cdr_tensor* ins, int n_in, const cdr_tensor* o
   CacheAttn a;
   bool empty = false;
   if (int rc = parse_prefix(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
-  return empty ? CDR_OK : run_cache_attention(a, ws, ws_bytes, stream);
+  return empty ? CDR_OK : run_cache_attention(a, "prefix_attention", ws, ws_bytes, stream);
 }
 
 }  // namespace cdr

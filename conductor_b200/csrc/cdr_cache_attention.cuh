@@ -47,6 +47,14 @@ struct PrefixPartials {
 // part.splits > 0: joined with the partial results; else the prefix is streamed as well.
 int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, cudaStream_t stream);
 
+// Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter.
+constexpr size_t kTileCounterBytes = 256;
+// prefix, sinks and window of every (sequence, query head), 256 queries per tile
+int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream);
+// the shared prefix alone, for G * Sq <= 128 query rows per sequence and key head, into *part in `ws`
+int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream);
+size_t packed_workspace(const CacheAttn& a);   // with the counter; 16-byte aligned start
+
 #ifdef __CUDACC__
 __device__ __forceinline__ int sequence_length(const CacheAttn& a, int b) {
   if (!a.lengths) return a.Skv;

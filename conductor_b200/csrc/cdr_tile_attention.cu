@@ -1,0 +1,654 @@
+// K8 -- attention over a key/value cache for many query rows: prompts and chunks of prompts (window and
+// prefix attention) and the shared prefix of a batch, whose rows are packed into one matrix product.
+//
+// Tensor-core bound.  The machine is that of cdr_attention.cu: persistent CTAs, one per SM; a tile is
+// 256 query rows in two 128-row halves that share every K/V block of 128 keys and take turns on the tensor
+// core; S = Q K^T (tcgen05, fp32 in tensor memory), softmax by one thread per row, P as 16-bit pairs
+// over the S columns, O += P V with P read from tensor memory; K and V through one 4-stage TMA ring.
+//   warp 0 TMA producer, warp 1 MMA issuer, warps 2-3 idle, warps 4-7 / 8-11 softmax of half A / B
+// (register split, barriers, reference-maximum rule: see that file).  What is different:
+//   - a tile walks a LIST of key blocks instead of a prefix of them: the shared prefix's blocks, the
+//     blocks that hold the sinks, then the blocks that its rows' windows touch.  Each half skips the blocks that
+//     none of its rows sees, so a window of W keys costs W / 128 + 2 blocks per half, wherever it lies.
+//   - query i stands at position L - Sq + i with L read per sequence by the producer warp, which hands it
+//     to the other warps with the tile index.  Masks are applied on the blocks at the edges only.
+//   - the cache behind L may hold anything: its scores are masked, and its V rows, which would turn a
+//     zero weight into NaN, are cleared in shared memory by the MMA warp (last block of a sequence only).
+//   - PACKED (shared prefix): the 128 rows of a half are the G*Sq rows of several sequences that share a key
+//     head, fetched by one 4-D box; the prefix is split over tiles and O / l and log2 of the sum go to
+//     scratch in fp32, where the streaming kernel joins them with the sequences' own keys.
+#include <cuda.h>
+#include <math.h>
+
+#include "cdr_attention_softmax.cuh"
+#include "cdr_cache_attention.cuh"
+#include "cdr_common.cuh"
+#include "cdr_sm100.cuh"
+
+namespace cdr {
+
+int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const int64_t* dims, const int64_t* strides,
+                       const int* box, bool swizzle);
+
+namespace {
+
+constexpr int HALF = 128, BQ = 256, BKV = 128;    // rows per half, per tile; keys per block
+constexpr int TA_THREADS = 384, SOFTMAX_WARP0 = 4;
+constexpr int REGS_CONTROL = 80, REGS_SOFTMAX = 208;   // 128*80 + 256*208 <= 384*168, the CTA's allocation at launch
+constexpr int TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;   // + 128 * half
+constexpr float kRescale = 8.0f;                  // log2 units
+constexpr int KV_STAGES = 4, TILE_SLOTS = 4, TILE_READERS = 9;
+
+struct TileArgs {
+  CUtensorMap tmap_q, tmap_k, tmap_v, tmap_pk, tmap_pv, tmap_o;
+  CacheAttn a;
+  unsigned int* next_tile;   // scratch: tiles handed out beyond the first per CTA (nullptr: there are none)
+  int* status;
+  int n_qtiles, group_heads, total_tiles;
+  // PACKED
+  int seqs_per_half, split_blocks, splits;
+  float *part_o, *part_lse;
+  int part_rows;
+};
+
+template <int HD>
+struct TileSmem {
+  static constexpr int TILE_BYTES = 128 * HD * 2;
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = 2 * TILE_BYTES;
+  static constexpr int BAR_OFF = KV_OFF + KV_STAGES * TILE_BYTES;
+  static constexpr int STAGE_OFF = BAR_OFF + 256;
+  static constexpr int STAGE_BYTES = 8 * 32 * 64;
+  static constexpr size_t TOTAL = STAGE_OFF + STAGE_BYTES + 1024;
+};
+
+enum { B_QFULL = 0, B_QEMPTY = 1, B_FULL = 2, B_EMPTY = B_FULL + KV_STAGES, B_SFULL = B_EMPTY + KV_STAGES, B_PFULL = B_SFULL + 2,
+       B_PVDONE = B_PFULL + 2, B_OFREE = B_PVDONE + 2, B_TFULL = B_OFREE + 2, B_TEMPTY = B_TFULL + TILE_SLOTS,
+       B_COUNT = B_TEMPTY + TILE_SLOTS };
+static_assert(B_COUNT * 8 + 8 + TILE_SLOTS * 8 <= 256, "barrier block");
+
+// One tile: its rows and its list of key blocks.  Entry j of the list is prefix block p0 + j for j < np, else
+// the sequence's own block own_block(j).
+struct Tile {
+  int b, hq, hkv, q0;        // sequence, heads, first query (PACKED: b is the first sequence of half A)
+  int off;                   // position of query 0
+  int p0, np;                // prefix blocks
+  int ns, wstart;            // own blocks: [0, ns) and [wstart, ...)
+  int n_iter;
+  int live[2], fw[2], lw[2]; // the half has rows that see keys; first and last own block of their windows
+
+  __device__ __forceinline__ int own_block(int j) const { const int o = j - np; return o < ns ? o : wstart + o - ns; }
+  __device__ __forceinline__ bool active(int h, int j) const {
+    if (!live[h]) return false;
+    if (j < np) return true;
+    const int kb = own_block(j);
+    return kb <= lw[h] && (kb < ns || kb >= fw[h]);
+  }
+};
+
+template <bool PACKED>
+__device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len, Tile& r) {
+  const CacheAttn& a = t.a;
+  if (PACKED) {
+    // row tiles innermost, then heads: the tiles in flight share the prefix's blocks in L2
+    const int rt = idx % t.n_qtiles, x = idx / t.n_qtiles;
+    r.hkv = x % a.Hkv;
+    const int split = x / a.Hkv;
+    r.b = rt * 2 * t.seqs_per_half;
+    r.hq = r.hkv * a.G;
+    r.q0 = 0;
+    r.off = split;
+    const int np = (a.P + BKV - 1) / BKV;
+    r.p0 = split * t.split_blocks;
+    r.np = min(t.split_blocks, np - r.p0);
+    r.ns = r.wstart = 0;
+    r.n_iter = r.np;
+    r.live[0] = 1;
+    r.live[1] = r.b + t.seqs_per_half < a.B;
+    return;
+  }
+  // heads in groups that fill the machine; inside a group the tiles from the last to the first, heads
+  // innermost: a key head's blocks are in L2 while its query heads and neighbouring tiles read them
+  const int BH = a.B * a.Hq;
+  const int per_group = t.group_heads * t.n_qtiles;
+  const int grp = idx / per_group, x = idx - grp * per_group;
+  const int hg = min(BH - grp * t.group_heads, t.group_heads);
+  const int bh = grp * t.group_heads + x % hg;
+  r.q0 = (t.n_qtiles - 1 - x / hg) * BQ;
+  r.b = bh / a.Hq;
+  r.hq = bh % a.Hq;
+  r.hkv = r.hq / a.G;
+  r.off = len - a.Sq;
+  int wlo = 0x7fffffff, whi = -1, p_max = -1;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row0 = r.q0 + h * HALF;
+    const int last = r.off + min(row0 + HALF, a.Sq) - 1;
+    r.live[h] = row0 < a.Sq && last >= 0;
+    r.fw[h] = max(max(r.off + row0, 0) - a.window + 1, 0) / BKV;
+    r.lw[h] = last / BKV;
+    if (r.live[h]) { wlo = min(wlo, r.fw[h]); whi = max(whi, r.lw[h]); p_max = max(p_max, last); }
+  }
+  r.p0 = r.np = r.ns = r.wstart = r.n_iter = 0;
+  if (p_max >= 0) {
+    r.np = (a.P + BKV - 1) / BKV;
+    r.ns = (min(a.sinks, p_max + 1) + BKV - 1) / BKV;
+    r.wstart = max(r.ns, wlo);
+    r.n_iter = r.np + r.ns + max(whi - r.wstart + 1, 0);
+  }
+}
+
+// tile_ring entry: index (-1: no more) and the sequence's length
+template <int HD, bool BF16, bool PACKED>
+__global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __grid_constant__ TileArgs t) {
+  using L = TileSmem<HD>;
+  const CacheAttn& a = t.a;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  volatile int* tile_ring = reinterpret_cast<volatile int*>(bars + B_COUNT + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    sm100::prefetch_tensormap(&t.tmap_q);
+    if (!PACKED) { sm100::prefetch_tensormap(&t.tmap_k); sm100::prefetch_tensormap(&t.tmap_v); sm100::prefetch_tensormap(&t.tmap_o); }
+    if (a.P > 0) { sm100::prefetch_tensormap(&t.tmap_pk); sm100::prefetch_tensormap(&t.tmap_pv); }
+    for (int i = 0; i < B_COUNT; ++i) {
+      const bool per_warp = (i >= B_PFULL && i < B_PFULL + 2) || (i >= B_OFREE && i < B_OFREE + 2);
+      const bool slot_free = i >= B_TEMPTY && i < B_TEMPTY + TILE_SLOTS;
+      sm100::mbar_init(&bars[i], slot_free ? TILE_READERS : per_warp ? 4 : 1);
+    }
+    sm100::fence_barrier_init();
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc(tmem_slot, TMEM_COLS);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  if (warp < SOFTMAX_WARP0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int ring = 0;
+      bool ok = true;
+      int idx = static_cast<int>(blockIdx.x);
+      for (int k = 0; ok; ++k) {
+        const int slot = k % TILE_SLOTS;
+        const bool valid = idx < t.total_tiles;
+        int len = 0;
+        if (!PACKED && valid) {
+          const int x = idx % (t.group_heads * t.n_qtiles), grp = idx / (t.group_heads * t.n_qtiles);
+          const int hg = min(a.B * a.Hq - grp * t.group_heads, t.group_heads);
+          len = sequence_length(a, (grp * t.group_heads + x % hg) / a.Hq);
+        }
+        if (k >= TILE_SLOTS && !sm100::mbar_wait(&bars[B_TEMPTY + slot], (k / TILE_SLOTS - 1) & 1)) { sm100::report_timeout(t.status, 40); break; }
+        tile_ring[2 * slot] = valid ? idx : -1;
+        tile_ring[2 * slot + 1] = len;
+        sm100::mbar_arrive(&bars[B_TFULL + slot]);
+        if (!valid) break;
+        Tile r;
+        decode_tile<PACKED>(t, idx, len, r);
+        idx = t.next_tile ? static_cast<int>(gridDim.x + atomicAdd(t.next_tile, 1u)) : t.total_tiles;
+        if (k > 0 && !sm100::mbar_wait(&bars[B_QEMPTY], (k - 1) & 1)) { sm100::report_timeout(t.status, 41); break; }
+        const int q_bytes = PACKED ? a.Sq * a.G * t.seqs_per_half * HD * 2 : L::TILE_BYTES;
+        sm100::mbar_arrive_expect_tx(&bars[B_QFULL], (r.live[0] + r.live[1]) * q_bytes);
+        for (int h = 0; h < 2; ++h)
+          if (r.live[h])
+#pragma unroll
+            for (int d = 0; d < HD / 64; ++d)
+              sm100::tma_load_4d(smem + L::Q_OFF + h * L::TILE_BYTES + d * (128 * 128), &t.tmap_q, d * 64,
+                                 PACKED ? 0 : r.q0 + h * HALF, r.hq, PACKED ? r.b + h * t.seqs_per_half : r.b, &bars[B_QFULL]);
+        for (int i = 0; i < 2 * r.n_iter; ++i) {      // K_j for i = 2j, V_j for i = 2j + 1
+          const int n = ring + i, st = n % KV_STAGES, use = n / KV_STAGES, j = i >> 1;
+          if (use > 0 && !sm100::mbar_wait(&bars[B_EMPTY + st], (use - 1) & 1)) { sm100::report_timeout(t.status, 42); ok = false; break; }
+          sm100::mbar_arrive_expect_tx(&bars[B_FULL + st], L::TILE_BYTES);
+          const bool pre = PACKED || j < r.np;
+          const void* tmap = pre ? ((i & 1) ? static_cast<const void*>(&t.tmap_pv) : static_cast<const void*>(&t.tmap_pk))
+                                 : ((i & 1) ? static_cast<const void*>(&t.tmap_v) : static_cast<const void*>(&t.tmap_k));
+          const int key0 = (pre ? r.p0 + j : r.own_block(j)) * BKV;
+#pragma unroll
+          for (int d = 0; d < HD / 64; ++d)
+            sm100::tma_load_4d(smem + L::KV_OFF + st * L::TILE_BYTES + d * (128 * 128), tmap, d * 64, key0, r.hkv, pre ? 0 : r.b,
+                               &bars[B_FULL + st]);
+        }
+        ring += 2 * r.n_iter;
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (convergent warp, elected lane)
+    const bool leader = sm100::elect_one();
+    constexpr uint32_t idesc_s = sm100::umma_idesc_f16(HALF, BKV, BF16, false, false);
+    constexpr uint32_t idesc_o = sm100::umma_idesc_f16(HALF, HD, BF16, false, true);  // V is MN-major
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+      const bool done = __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity));
+      if (!done && leader) sm100::report_timeout(t.status, site);
+      return done;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) sm100::umma_commit(bar);
+      __syncwarp();
+    };
+    int ring = 0;
+    int blocks[2] = {0, 0};       // key blocks issued so far per half (phases of its P barrier)
+    int tiles_done[2] = {0, 0};   // tiles with at least one product issued, per half (gates the reuse of O_h)
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int slot = k % TILE_SLOTS;
+      ok = wait_all(&bars[B_TFULL + slot], (k / TILE_SLOTS) & 1, 43);
+      if (!ok) break;
+      const int idx = tile_ring[2 * slot], len = tile_ring[2 * slot + 1];
+      __syncwarp();
+      if (leader) sm100::mbar_arrive(&bars[B_TEMPTY + slot]);
+      if (idx < 0) break;
+      Tile r;
+      decode_tile<PACKED>(t, idx, len, r);
+      const int n_iter = r.n_iter;
+      ok = wait_all(&bars[B_QFULL], k & 1, 44);
+      if (!ok) break;
+      auto ring_wait = [&](int i, int site) { const int n = ring + i; return wait_all(&bars[B_FULL + n % KV_STAGES], (n / KV_STAGES) & 1, site); };
+      auto ring_free = [&](int i) { commit(&bars[B_EMPTY + (ring + i) % KV_STAGES]); };
+      auto issue_s = [&](int h, int j) {
+        const uint32_t q_addr = sm100::smem_u32(smem + L::Q_OFF + h * L::TILE_BYTES);
+        const uint32_t k_addr = sm100::smem_u32(smem + L::KV_OFF + ((ring + 2 * j) % KV_STAGES) * L::TILE_BYTES);
+        const uint32_t d = tmem_base + TMEM_S + h * 128;
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t o = (kk / 4) * (128 * 128) + (kk % 4) * 32;
+            sm100::umma_f16_ss(d, sm100::umma_desc_k_sw128(q_addr + o), sm100::umma_desc_k_sw128(k_addr + o), idesc_s, kk > 0 ? 1u : 0u);
+          }
+          sm100::umma_commit(&bars[B_SFULL + h]);
+        }
+        __syncwarp();
+      };
+      bool started[2] = {false, false};
+      if (n_iter > 0) {
+        ok = ring_wait(0, 45);
+        if (!ok) break;
+        sm100::tc_fence_after();
+        for (int h = 0; h < 2; ++h)
+          if (r.active(h, 0)) issue_s(h, 0);
+        ring_free(0);
+      }
+      if (n_iter <= 1) commit(&bars[B_QEMPTY]);
+      for (int j = 0; j < n_iter && ok; ++j) {
+        const bool next = j + 1 < n_iter;
+        const int vt = 2 * j + 1, kt = 2 * j + 2;
+        ok = ring_wait(vt, 46);
+        if (!ok) break;
+        bool k_ready = false;
+        unsigned char* v_tile = smem + L::KV_OFF + ((ring + vt) % KV_STAGES) * L::TILE_BYTES;
+        const uint32_t v_addr = sm100::smem_u32(v_tile);
+        if (!PACKED && j >= r.np) {
+          // V rows behind the sequence's end: a weight of 0 must not meet what the cache holds there
+          const int keep = len - r.own_block(j) * BKV;
+          if (keep < BKV && len < a.Skv) {
+            for (int x = lane; x < (BKV - keep) * (HD / 8); x += 32) {
+              const int row = keep + x / (HD / 8), piece = x % (HD / 8);
+              *reinterpret_cast<uint4*>(v_tile + (piece >> 3) * (128 * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (r.active(h, j)) {
+            if (!started[h] && tiles_done[h] > 0) {    // the previous tile's epilogue must have read O_h
+              ok = wait_all(&bars[B_OFREE + h], (tiles_done[h] - 1) & 1, 47);
+              if (!ok) break;
+            }
+            ok = wait_all(&bars[B_PFULL + h], blocks[h] & 1, 48 + h);
+            if (!ok) break;
+            ++blocks[h];
+            sm100::tc_fence_after();
+            const uint32_t p_tmem = tmem_base + TMEM_S + h * 128;
+            if (leader) {
+              const uint32_t acc = started[h] ? 1u : 0u;
+#pragma unroll
+              for (int kk = 0; kk < BKV / 16; ++kk)
+                sm100::umma_f16_ts(tmem_base + TMEM_O + h * 128, p_tmem + kk * 8, sm100::umma_desc_mn_sw128(v_addr + kk * (16 * 128), 128 * 128),
+                                   idesc_o, kk > 0 ? 1u : acc);
+              sm100::umma_commit(&bars[B_PVDONE + h]);
+            }
+            __syncwarp();
+            if (!started[h]) { started[h] = true; ++tiles_done[h]; }
+          }
+          if (next && r.active(h, j + 1)) {
+            if (!k_ready) {
+              ok = ring_wait(kt, 50);
+              if (!ok) break;
+              k_ready = true;
+              sm100::tc_fence_after();
+            }
+            issue_s(h, j + 1);
+          }
+        }
+        if (!ok) break;
+        ring_free(vt);
+        if (next) {
+          if (!k_ready && !(ok = ring_wait(kt, 50))) break;   // a stage is handed back only after it was filled
+          ring_free(kt);
+        }
+        if (j + 2 == n_iter) commit(&bars[B_QEMPTY]);
+      }
+      ring += 2 * n_iter;
+    }
+  } else if (warp >= SOFTMAX_WARP0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    // ------------------------------------------------------------ softmax / correction / epilogue
+    const int g = (warp - SOFTMAX_WARP0) >> 2;       // half this warp group serves
+    const int q = warp & 3;                          // tensor-memory lane quadrant
+    const int row_in_half = q * 32 + lane;
+    const uint32_t lane_sel = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t s_taddr = tmem_base + TMEM_S + g * 128 + lane_sel;
+    const uint32_t o_taddr = tmem_base + TMEM_O + g * 128 + lane_sel;
+    unsigned char* stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * (32 * 64);
+    int n = 0;                                       // key blocks consumed so far over all tiles
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int slot = k % TILE_SLOTS;
+      if (!sm100::mbar_wait(&bars[B_TFULL + slot], (k / TILE_SLOTS) & 1)) { sm100::report_timeout(t.status, 51); break; }
+      const int idx = tile_ring[2 * slot], len = tile_ring[2 * slot + 1];
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&bars[B_TEMPTY + slot]);
+      if (idx < 0) break;
+      Tile r;
+      decode_tile<PACKED>(t, idx, len, r);
+      const int row0 = r.q0 + g * HALF;
+      const int p_first = r.off + row0, p_last = r.off + min(row0 + HALF, a.Sq) - 1;
+      const int pos = p_first + row_in_half;         // this row's position (PACKED: unused)
+      float m_ref = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+      bool first = true;
+
+      for (int j = 0; j < r.n_iter; ++j) {
+        if (!r.active(g, j)) continue;
+        if (!sm100::mbar_wait(&bars[B_SFULL + g], n & 1)) { sm100::report_timeout(t.status, 52); ok = false; break; }
+        ++n;
+        sm100::tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sm100::tmem_ld32(s_taddr + c * 32, sr[c]);
+        sm100::tmem_ld_wait();
+
+        if (PACKED || j < r.np) {
+          const int left = a.P - (r.p0 + j) * BKV;   // keys of the prefix from here on
+          if (left < BKV) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i >= left) sr[c][i] = __float_as_uint(-INFINITY);
+          }
+        } else {
+          const int key0 = r.own_block(j) * BKV;
+          if (key0 + BKV - 1 > p_first) {            // keys behind some row (behind the end too: p < len)
+            const int see = pos - key0;              // visible: i <= see
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i > see) sr[c][i] = __float_as_uint(-INFINITY);
+          }
+          if (key0 <= p_last - a.window && key0 + BKV > a.sinks) {   // keys in front of some row's window
+            const int gone = pos - a.window - key0, sink = a.sinks - key0;   // hidden: i <= gone and i >= sink
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i <= gone && c * 32 + i >= sink) sr[c][i] = __float_as_uint(-INFINITY);
+          }
+        }
+
+        if (first) {
+          first = false;
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              mx[i & 3] = max3(mx[i & 3], __uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1]));
+          m_ref = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+          store_p<BF16, 0, false>(sr, a.scale_log2, neg_m, l0, l1, s_taddr);
+        } else {
+          float l0s = l0, l1s = l1;
+          const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+          const float bmax = store_p<BF16, 0, true>(sr, a.scale_log2, neg_m, l0s, l1s, s_taddr) * a.scale_log2;
+          if (__any_sync(0xffffffffu, bmax > m_ref + kRescale)) {
+            const float m_new = fmaxf(m_ref, bmax);
+            const float alpha = (m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
+            l0 *= alpha;
+            l1 *= alpha;
+            m_ref = m_new;
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              sm100::tmem_ld32(o_taddr + c * 32, o);
+              sm100::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              sm100::tmem_st32(o_taddr + c * 32, o);
+            }
+            sm100::tmem_st_wait();
+            const float neg_m2 = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+            store_p<BF16, 0, false>(sr, a.scale_log2, neg_m2, l0, l1, s_taddr);
+          } else {
+            l0 = l0s;
+            l1 = l1s;
+          }
+        }
+        sm100::tmem_st_wait();
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&bars[B_PFULL + g]);
+      }
+      if (!ok) break;
+
+      // ---- epilogue: O / l; O_h is handed back after the last read
+      if (!r.live[g] && (PACKED || row0 >= a.Sq)) continue;
+      const float l = l0 + l1;
+      const bool none = !r.live[g] || (!PACKED && pos < 0) || l == 0.0f;
+      const float inv = 1.0f / l;
+      if (r.live[g]) {
+        if (!sm100::mbar_wait(&bars[B_PVDONE + g], (n - 1) & 1)) { sm100::report_timeout(t.status, 53); ok = false; break; }
+        sm100::tc_fence_after();
+      }
+      if constexpr (PACKED) {
+        const int per_seq = a.G * a.Sq, bb = row_in_half / per_seq, rem = row_in_half - bb * per_seq;
+        const int b = r.b + g * t.seqs_per_half + bb;
+        const bool write = bb < t.seqs_per_half && b < a.B;
+        const size_t prow = (static_cast<size_t>(b) * a.Sq + rem % a.Sq) * a.G + rem / a.Sq;
+        const size_t at = (static_cast<size_t>(r.off) * a.Hkv + r.hkv) * t.part_rows + prow;
+        if (write) t.part_lse[at] = none ? -INFINITY : m_ref + __log2f(l);
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          sm100::tmem_ld32(o_taddr + c * 32, o);
+          sm100::tmem_ld_wait();
+          if (c == HD / 32 - 1) {
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&bars[B_OFREE + g]);
+          }
+          if (write) {
+            float4* dst = reinterpret_cast<float4*>(t.part_o + at * HD + c * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = none ? make_float4(0, 0, 0, 0)
+                            : make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                          __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t w[16];
+          if (r.live[g]) {
+            uint32_t o[32];
+            sm100::tmem_ld32(o_taddr + c * 32, o);
+            sm100::tmem_ld_wait();
+            if (c == HD / 32 - 1) {
+              sm100::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) sm100::mbar_arrive(&bars[B_OFREE + g]);
+            }
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              w[x] = none ? 0u : pack_pair<BF16>(__uint_as_float(o[x * 2]) * inv, __uint_as_float(o[x * 2 + 1]) * inv);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) w[x] = 0u;    // a half of padding: nothing was computed
+          }
+          if (lane == 0) sm100::bulk_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + x * 16) = make_uint4(w[x * 4], w[x * 4 + 1], w[x * 4 + 2], w[x * 4 + 3]);
+          sm100::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            sm100::tma_store_4d(&t.tmap_o, stage, c * 32, row0 + q * 32, r.hq, r.b);
+            sm100::bulk_commit();
+          }
+        }
+      }
+    }
+    if (!PACKED && lane == 0) sm100::bulk_wait<0>();
+  }
+
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+template <int HD, bool BF16, bool PACKED>
+int launch_tile_cfg(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stream) {
+  auto kern = tile_attention_kernel<HD, BF16, PACKED>;
+  constexpr size_t smem = TileSmem<HD>::TOTAL;
+  static bool configured_dev[64] = {false};
+  int dev = 0;
+  CDR_CUDA_TRY(cudaGetDevice(&dev));
+  if (!configured_dev[dev & 63]) {
+    // setmaxnreg.inc waits until the CTA's registers at launch cover the split: refuse a build that got fewer
+    cudaFuncAttributes fa;
+    CDR_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
+    if (fa.numRegs * TA_THREADS < 128 * REGS_CONTROL + (TA_THREADS - 128) * REGS_SOFTMAX) {
+      set_error("attention: kernel was built with %d registers per thread, fewer than its register split needs", fa.numRegs);
+      return CDR_ERR_UNSUPPORTED;
+    }
+    CDR_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    configured_dev[dev & 63] = true;
+  }
+  t.total_tiles = static_cast<int>(tiles);
+  t.status = device_status_ptr();
+  const int64_t sms = sm_count();
+  const int64_t grid = tiles < sms ? tiles : sms;
+  t.next_tile = nullptr;
+  if (tiles > grid) {            // CTAs draw tiles beyond their first from a counter
+    t.next_tile = static_cast<unsigned int*>(counter);
+    CDR_CUDA_TRY(cudaMemsetAsync(t.next_tile, 0, sizeof(unsigned int), stream));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(TA_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, t));
+  return CDR_OK;
+}
+
+template <bool PACKED>
+int launch_tile_typed(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stream) {
+  if (tiles > 0x3fffffff) { set_error("attention: too many tiles"); return CDR_ERR_UNSUPPORTED; }
+  if (t.a.D == 128) return t.a.bf16 ? launch_tile_cfg<128, true, PACKED>(t, tiles, counter, stream) : launch_tile_cfg<128, false, PACKED>(t, tiles, counter, stream);
+  return t.a.bf16 ? launch_tile_cfg<64, true, PACKED>(t, tiles, counter, stream) : launch_tile_cfg<64, false, PACKED>(t, tiles, counter, stream);
+}
+
+int map_heads(CUtensorMap* m, const void* base, const CacheAttn& a, int64_t S, int64_t H, int64_t B, const HeadStrides& st, int box_d,
+              int box_s, int box_h, int box_b, bool swizzle) {
+  const int64_t dims[4] = {a.D, S, H, B}, strides[3] = {st.s, st.h, st.b};
+  const int box[4] = {box_d, box_s, box_h, box_b};
+  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, swizzle);
+}
+
+int map_prefix(TileArgs& t) {
+  const CacheAttn& a = t.a;
+  if (a.P == 0) return CDR_OK;
+  HeadStrides pk = a.spk, pv = a.spv;
+  pk.b = pv.b = a.D;             // one "sequence": the stride is never used
+  if (int rc = map_heads(&t.tmap_pk, a.pk, a, a.P, a.Hkv, 1, pk, 64, BKV, 1, 1, true)) return rc;
+  return map_heads(&t.tmap_pv, a.pv, a, a.P, a.Hkv, 1, pv, 64, BKV, 1, 1, true);
+}
+
+}  // namespace
+
+int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
+  TileArgs t = {};
+  t.a = a;
+  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, HALF, 1, 1, true)) return rc;
+  if (int rc = map_heads(&t.tmap_o, a.out, a, a.Sq, a.Hq, a.B, a.so, 32, 32, 1, 1, false)) return rc;
+  if (a.Skv > 0) {               // an empty cache is never loaded from
+    if (int rc = map_heads(&t.tmap_k, a.k, a, a.Skv, a.Hkv, a.B, a.sk, 64, BKV, 1, 1, true)) return rc;
+    if (int rc = map_heads(&t.tmap_v, a.v, a, a.Skv, a.Hkv, a.B, a.sv, 64, BKV, 1, 1, true)) return rc;
+  }
+  if (int rc = map_prefix(t)) return rc;
+  t.n_qtiles = (a.Sq + BQ - 1) / BQ;
+  const int64_t BH = static_cast<int64_t>(a.B) * a.Hq;
+  if (BH * t.n_qtiles > 0x3fffffff) { set_error("attention: too many tiles"); return CDR_ERR_UNSUPPORTED; }
+  const int fill = sm_count() / t.n_qtiles;
+  t.group_heads = static_cast<int>(fill < 1 ? 1 : fill > BH ? BH : fill);
+  return launch_tile_typed<false>(t, BH * t.n_qtiles, ws, stream);
+}
+
+// How the shared prefix is cut for the packed product: sequences per half, row tiles, key splits.
+void plan_packed(const CacheAttn& a, int* seqs_per_half, int* row_tiles, int* split_blocks, int* splits) {
+  const int per_seq = a.G * a.Sq;
+  const int fit = HALF / per_seq;
+  *seqs_per_half = fit < a.B ? fit : a.B;
+  *row_tiles = (a.B + 2 * *seqs_per_half - 1) / (2 * *seqs_per_half);
+  const int blocks = (a.P + BKV - 1) / BKV;
+  const int64_t tasks = static_cast<int64_t>(a.Hkv) * *row_tiles;
+  int64_t n = sm_count() / tasks;
+  n = n < 1 ? 1 : n > blocks ? blocks : n;
+  *split_blocks = static_cast<int>((blocks + n - 1) / n);
+  *splits = (blocks + *split_blocks - 1) / *split_blocks;
+}
+
+size_t packed_workspace(const CacheAttn& a) {
+  int seqs, tiles, blocks, splits;
+  plan_packed(a, &seqs, &tiles, &blocks, &splits);
+  const size_t rows = static_cast<size_t>(a.B) * a.Sq * a.G;
+  return kTileCounterBytes + static_cast<size_t>(splits) * a.Hkv * rows * (a.D + 1) * sizeof(float);
+}
+
+int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream) {
+  TileArgs t = {};
+  t.a = a;
+  plan_packed(a, &t.seqs_per_half, &t.n_qtiles, &t.split_blocks, &t.splits);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.G;
+  t.part_rows = static_cast<int>(rows);
+  t.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kTileCounterBytes);
+  t.part_lse = t.part_o + static_cast<size_t>(t.splits) * a.Hkv * rows * a.D;
+  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, a.Sq, a.G, t.seqs_per_half, true)) return rc;
+  if (int rc = map_prefix(t)) return rc;
+  *part = PrefixPartials{t.part_o, t.part_lse, t.splits, t.part_rows};
+  return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, ws, stream);
+}
+
+}  // namespace cdr

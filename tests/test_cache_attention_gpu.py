@@ -198,6 +198,26 @@ def test_other_streams_and_graph_replay():
     assert all(torch.equal(a, b) for a, b in zip(graphs[0][1], calls()))
 
 
+def test_more_tiles_than_processors_in_a_graph():
+    """Tiles are drawn from a counter in scratch: every replay starts it again, on each of two graphs at once."""
+    q, k, v = cache(20, 8, 2, 300, 300, 64)
+    n = torch.arange(20, device=DEV) * 17
+    want = WINDOW(q, k, v, 100, 4, lengths=n)
+    check(want, reference(q, k, v, window=100, sinks=4, lengths=n))
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = WINDOW(q, k, v, 100, 4, lengths=n)
+        graphs.append((g, out))
+    for _ in range(4):
+        for s, (g, _o) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _g, out in graphs)
+
+
 def test_the_same_call_gives_the_same_bits():
     q, k, v = cache(3, 8, 2, 2, 999, 128)
     pre = [rand(2, 2000, 128, seed=50 + i) for i in range(2)]
