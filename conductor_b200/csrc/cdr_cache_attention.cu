@@ -4,23 +4,26 @@
 // CDR_T_WINDOW_ATTENTION and CDR_T_PREFIX_ATTENTION.  The reference has no attention over a cache;
 // its kernels (choreo-op/attention-gcu-only-test.co:15-134) take q, k and v of one length.
 //
-// HBM bound: every visible key and value is read once for the (at most 16) rows of a task.  The
-// keys of a task are split over the warps of a thread-block cluster (4 warps per CTA, 1 to 16 CTAs),
-// each warp running the online-softmax recurrence over blocks of 16 keys on its own:
-//   - K and V go from global memory straight into the operand registers of m16n8k16 matrix
-//     instructions.  The order of the contraction index is free as long as both operands use the
-//     same one, so a thread takes 16 contiguous bytes of a K row (and of the Q row) for two
-//     k-steps; for P V it takes 16 bytes of four V rows and pairs them with byte permutes.  No
-//     shared memory, no barrier in the loop.  16 rows are the instruction's height: a task with
-//     fewer rows pays nothing for it, the loads set the pace.
-//   - the K registers are reloaded for the next block right behind the score products, the V
-//     registers behind the output products: a warp keeps 4 to 8 KB in flight (HD = 128).
+// HBM bound: every visible key and value is read once for the (at most 16) rows of a task, a task being
+// (sequence, key head, 16-row tile).  The work of all tasks is one list of units of 32 keys, cut into equal
+// contiguous shares, one per warp of a grid that is resident as a whole: whatever the lengths, all warps
+// finish together.  Each warp runs the online-softmax recurrence on its own, without a barrier:
+//   - the TMA unit brings K and V of a unit into the warp's own two-stage ring (16 KB per stage at HD = 128,
+//     192 KB in flight per SM); copying them with per-thread 16-byte asynchronous copies instead was
+//     bound by instructions and shared-memory traffic at 4.1 TB/s (440 instructions per 16 keys).
+//   - the 16-byte pieces are operand registers of m16n8k16 matrix instructions as they are: the order of the
+//     contraction index is free as long as both operands use the same one, so a lane takes a piece of a K
+//     row (and of the Q row) for two k-steps; for P V it takes a piece of four V rows and pairs them with byte
+//     permutes.  With the 128-byte swizzle, lanes c = 0..3 reading pieces 2c + j of a K row, and eight lanes a
+//     whole V row, meet no bank conflict.  16 rows are the instruction's height: a task with fewer rows
+//     pays nothing for it, the loads set the pace.
 //   - the accumulator is rescaled only when a row's maximum grew by more than 2^8; exact after the
 //     final division because the sums use the same reference.
-// The warps' (maximum, sum, O) are joined in shared memory, the CTAs' through distributed shared
-// memory, each CTA writing 16 / cluster-size rows: one launch, no scratch, no atomics, and the order
-// of the sums is fixed.  P is rounded to the input type for the second product (relative 2^-9 per
-// weight at bf16, independent per key); scores, maxima, sums and O stay in fp32.
+// A warp that has all units of a task writes the output, otherwise (maximum, sum, O) in fp32 to scratch; a
+// second kernel, launched to overlap this one's tail, adds up each row's parts in the order of the keys (no
+// atomics: the same call gives the same bits) and those of the shared prefix (cdr_tile_attention.cu).
+// P is rounded to the input type for the second product (relative 2^-9 per weight at bf16, independent per
+// key); scores, maxima, sums and O stay in fp32.
 #include <cuda.h>
 #include <math.h>
 
@@ -28,19 +31,34 @@
 #include "cdr_sm100.cuh"
 
 namespace cdr {
+
+int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const int64_t* dims, const int64_t* strides,
+                       const int* box, bool swizzle);
+
 namespace {
 
-constexpr int SA_WARPS = 4;          // per CTA; they split the keys
 constexpr int SA_ROWS = 16;          // query rows of a task (m of the matrix instruction)
-constexpr int SA_KEYS = 16;          // keys per block (k of the second product)
-constexpr int SA_MAX_CLUSTER = 16;
+constexpr int SA_KEYS = 32;          // keys per unit
+constexpr int SA_STAGES = 2;         // units in flight per warp
+constexpr int SA_GROUPS = 2048;      // entries of the table of cumulated units
 constexpr float SA_RESCALE = 8.0f;   // log2 units
 
+int make_map(CUtensorMap* m, const void* base, const CacheAttn& a, int64_t S, int64_t H, int64_t B, const HeadStrides& st) {
+  const int64_t dims[4] = {a.D, S, H, B}, strides[3] = {st.s, st.h, st.b};
+  const int box[4] = {64, SA_KEYS, 1, 1};
+  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, true);
+}
+
 struct StreamArgs {
+  CUtensorMap tmap_k, tmap_v, tmap_pk, tmap_pv;   // [B, H, S, D] and the prefix as one sequence; box 64 x 32 keys
   CacheAttn a;
-  PrefixPartials part;
-  int m_tiles;        // tasks per (sequence, key head)
-  int cluster;
+  int* status;
+  PrefixPartials part;     // splits > 0: the prefix is already done
+  float *slot_o, *slot_ml; // parts: [slot][row of the task][D] and [..][2] = (maximum, sum)
+  int n_warps;             // shares
+  int m_tiles;             // tasks per (sequence, key head)
+  int group, groups;       // sequences per table entry, table entries
+  int rows_cap;            // rows of a slot: min(16, G * Sq)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -68,360 +86,634 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
-// a cached key is read by the CTAs of one task (and of the other row tiles of its head) only
-__device__ __forceinline__ uint4 ld_cache16(const unsigned char* p) {
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
   return r;
 }
 
-// The keys a task reads, as up to three ranges of blocks of 16: prefix, sinks, window.
+// The keys a task reads, as up to three ranges of units of 16: prefix, sinks, window.
 struct KeyRanges {
-  int n_prefix, n_sink, n_total;   // block counts (cumulative)
   int prefix_end, sink_end, lo, hi;
+  int n_prefix, n_sink, n_total;   // units, cumulated
+  bool one_position;               // the live rows see exactly the keys of the ranges
 };
 
-struct Block {
-  const unsigned char *k, *v;      // row 0 of the source
-  int64_t ks, vs;                  // row pitch in bytes
-  int base, end;                   // first key, one past the last key that may be read
-  int own;                         // the sequence's own keys (masked by position), not the prefix
-};
+__host__ __device__ __forceinline__ int min_(int a, int b) { return a < b ? a : b; }
+__host__ __device__ __forceinline__ int max_(int a, int b) { return a > b ? a : b; }
 
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(SA_WARPS * 32, 3) stream_attention_kernel(const __grid_constant__ StreamArgs args) {
-  constexpr int KC = HD / 32;      // 16-byte chunks of a K row per thread
-  constexpr int VC = HD / 64;      // 16-byte chunks of a V row per thread
-  constexpr int PITCH = HD + 4;
-  __shared__ __align__(16) float sm_o[SA_WARPS][SA_ROWS][PITCH];
-  __shared__ float sm_m[SA_WARPS][SA_ROWS], sm_l[SA_WARPS][SA_ROWS];
-  const CacheAttn& a = args.a;
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c = lane & 3;
-  const int cs = args.cluster;
-  const int rank = blockIdx.x % cs;            // == %cluster_ctarank: the cluster is 1-D along x
-  int task = blockIdx.x / cs;
-  const int mt = task % args.m_tiles; task /= args.m_tiles;
-  const int hkv = task % a.Hkv, b = task / a.Hkv;
-
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  const int len = sequence_length(a, b);
-  const int off = len - a.Sq;                  // position of query 0
-  const int rows = a.G * a.Sq;                 // row r = i * G + g: a tile spans few positions
-  const int r_first = mt * SA_ROWS, r_last = min(r_first + SA_ROWS, rows) - 1;
-  const int p_last = off + r_last / a.G;
-  const int p_first = max(off + r_first / a.G, 0);   // first row of the tile that sees keys
-
+__host__ __device__ __forceinline__ KeyRanges key_ranges(const CacheAttn& a, int prefix, int len, int mt) {
   KeyRanges kr;
-  kr.lo = kr.hi = kr.sink_end = kr.prefix_end = 0;
+  kr.prefix_end = kr.sink_end = kr.lo = kr.hi = 0;
+  const int off = len - a.Sq;
+  const int r_first = mt * SA_ROWS, r_last = min_(r_first + SA_ROWS, a.G * a.Sq) - 1;   // row r = i * G + g
+  const int p_last = off + r_last / a.G, p_first = max_(off + r_first / a.G, 0);        // first row that sees keys
   if (p_last >= 0) {
+    kr.prefix_end = prefix;
     kr.hi = p_last + 1;
-    kr.lo = max(p_first - a.window + 1, 0);
-    kr.sink_end = min(a.sinks, kr.lo);
-    if (args.part.splits == 0) kr.prefix_end = a.P;
+    kr.lo = max_(p_first - a.window + 1, 0);
+    kr.sink_end = min_(a.sinks, kr.lo);
   }
+  kr.one_position = p_first == p_last;
   kr.n_prefix = (kr.prefix_end + SA_KEYS - 1) / SA_KEYS;
   kr.n_sink = kr.n_prefix + (kr.sink_end + SA_KEYS - 1) / SA_KEYS;
   kr.n_total = kr.n_sink + (kr.hi - kr.lo + SA_KEYS - 1) / SA_KEYS;
+  return kr;
+}
 
-  const unsigned char* k_own = static_cast<const unsigned char*>(a.k) + (b * a.sk.b + hkv * a.sk.h) * 2;
-  const unsigned char* v_own = static_cast<const unsigned char*>(a.v) + (b * a.sv.b + hkv * a.sv.h) * 2;
-  const unsigned char* k_pre = static_cast<const unsigned char*>(a.pk) + hkv * a.spk.h * 2;
-  const unsigned char* v_pre = static_cast<const unsigned char*>(a.pv) + hkv * a.spv.h * 2;
+// units of one key head of a sequence
+__host__ __device__ __forceinline__ int head_units(const CacheAttn& a, int prefix, int len, int m_tiles) {
+  int n = 0;
+  for (int mt = 0; mt < m_tiles; ++mt) n += key_ranges(a, prefix, len, mt).n_total;
+  return n;
+}
 
-  auto block_of = [&](int t) {
-    Block x;
-    if (t < kr.n_prefix) {
-      x = Block{k_pre, v_pre, a.spk.s * 2, a.spv.s * 2, t * SA_KEYS, kr.prefix_end, 0};
-    } else if (t < kr.n_sink) {
-      x = Block{k_own, v_own, a.sk.s * 2, a.sv.s * 2, (t - kr.n_prefix) * SA_KEYS, kr.sink_end, 1};
-    } else {
-      x = Block{k_own, v_own, a.sk.s * 2, a.sv.s * 2, kr.lo + (t - kr.n_sink) * SA_KEYS, kr.hi, 1};
+struct Task {
+  int b, hkv, mt, len;
+  int first, units;      // its first unit in the list, and how many it has
+  KeyRanges kr;
+};
+
+// The task that unit u of the list belongs to.
+__device__ __forceinline__ Task find_task(const StreamArgs& s, const int* cum, int uniform, int u) {
+  const CacheAttn& a = s.a;
+  const int prefix = s.part.splits == 0 ? a.P : 0;
+  Task t;
+  int rest, per_head;
+  if (uniform) {                       // no lengths: every sequence has the same units
+    per_head = uniform;
+    t.b = u / (uniform * a.Hkv);
+    rest = u - t.b * (uniform * a.Hkv);
+    t.len = a.Skv;
+  } else {
+    int lo = 0, hi = s.groups - 1;     // last entry with cum <= u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    return x;
-  };
+    t.b = lo * s.group;
+    rest = u - cum[lo];
+    for (;;) {
+      t.len = sequence_length(a, t.b);
+      per_head = head_units(a, prefix, t.len, s.m_tiles);
+      if (rest < per_head * a.Hkv) break;
+      rest -= per_head * a.Hkv;
+      ++t.b;
+    }
+  }
+  t.hkv = rest / per_head;
+  rest -= t.hkv * per_head;
+  for (t.mt = 0;; ++t.mt) {
+    t.kr = key_ranges(a, prefix, t.len, t.mt);
+    if (rest < t.kr.n_total) break;
+    rest -= t.kr.n_total;
+  }
+  t.first = u - rest;
+  t.units = t.kr.n_total;
+  return t;
+}
 
-  // this thread's two query rows: g and g + 8 of the tile
+// Equal shares of the list: share w starts at begin(w); unit u is in share of(u).
+struct Shares {
+  int n, per, more;      // the first `more` shares have per + 1 units
+  __device__ __forceinline__ Shares(int total, int warps) {
+    n = min(warps, max(total, 1));     // no share in between is empty
+    per = total / n;
+    more = total - per * n;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * per + min(w, more); }
+  __device__ __forceinline__ int of(int u) const {
+    const int split = more * (per + 1);
+    return u < split ? u / (per + 1) : more + (u - split) / per;
+  }
+};
+
+// The list of units: cum[e] = units in front of table entry e (lengths given); returns their total, and the units
+// of a key head where every sequence has the same.  All THREADS threads of the block take part.
+template <int THREADS>
+__device__ __forceinline__ int cumulate_units(const StreamArgs& s, int* cum, int* warp_sum, int* uniform) {
+  const CacheAttn& a = s.a;
+  const int prefix = s.part.splits == 0 ? a.P : 0;
+  *uniform = 0;
+  if (!a.lengths) {
+    *uniform = head_units(a, prefix, a.Skv, s.m_tiles);
+    return *uniform * a.Hkv * a.B;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int e0 = 0; e0 < s.groups; e0 += THREADS) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    int n = 0;
+    if (e < s.groups)
+      for (int b = e * s.group; b < min(a.B, (e + 1) * s.group); ++b)
+        n += head_units(a, prefix, sequence_length(a, b), s.m_tiles) * a.Hkv;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) x += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (e < s.groups) cum[e] = carry + x - n;
+    carry += all;
+    __syncthreads();
+  }
+  return carry;
+}
+
+// what a staged unit is (written with its copies, read when it is used)
+struct __align__(16) UnitHeader {
+  int base, end;         // first key; one past the last key that may be used
+  int flags;             // 1: masked by position  2: starts a segment  4: ends one  8: its task lies in this share as a whole
+  int b, hkv, mt, off, task_first;
+};
+
+// 6 warps at HD = 128, 12 at HD = 64, where a unit has half the bytes and about as many dependent steps.
+template <int HD>
+struct StreamSmem {
+  static constexpr int WARPS = HD == 128 ? 6 : 12;
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int HALF_BYTES = SA_KEYS * HD * 2;          // K or V of a unit
+  static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr int HEAD_OFF = WARPS * SA_STAGES * STAGE_BYTES;
+  static constexpr int BAR_OFF = HEAD_OFF + WARPS * SA_STAGES * static_cast<int>(sizeof(UnitHeader));
+  static constexpr int CUM_OFF = BAR_OFF + WARPS * SA_STAGES * 8;
+  static constexpr int FIXED = CUM_OFF + 1024;                 // alignment slack
+};
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_kernel(const __grid_constant__ StreamArgs args) {
+  using L = StreamSmem<HD>;
+  constexpr int AC = HD / 64;      // 64-column atoms of a row: 128 bytes, 8 pieces
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* cum = reinterpret_cast<int*>(smem + L::CUM_OFF);
+  __shared__ int warp_sum[L::WARPS];
+  const CacheAttn& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  UnitHeader* heads = reinterpret_cast<UnitHeader*>(smem + L::HEAD_OFF) + warp * SA_STAGES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF) + warp * SA_STAGES;
+  unsigned char* ring = smem + warp * (SA_STAGES * L::STAGE_BYTES);
+  if (lane == 0) {
+    if (a.Skv > 0) { sm100::prefetch_tensormap(&args.tmap_k); sm100::prefetch_tensormap(&args.tmap_v); }
+    for (int st = 0; st < SA_STAGES; ++st) sm100::mbar_init(&bars[st], 1);
+    sm100::fence_barrier_init();
+  }
+  __syncwarp();
+
+  // Behind the packed prefix product this kernel needs nothing of that one, only what came before it, and that one
+  // lets its dependents start after its own wait: the wait for it is at the end, for the kernel that adds up.
+  const bool behind_prefix = args.part.splits > 0;
+  if (!behind_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  int uniform;
+  const int total = cumulate_units<L::THREADS>(args, cum, warp_sum, &uniform);
+  const Shares shares(total, args.n_warps);
+  const int share = warp * gridDim.x + blockIdx.x;       // neighbouring shares on different SMs
+  const int u_begin = share < shares.n ? shares.begin(share) : 0;
+  const int u_end = share < shares.n ? shares.begin(share + 1) : 0;
+
+  // ---- loads run ahead of their use: unit `lu`, in the segment of its task that ends at unit `seg_end`
+  int lu = u_begin, seg_end = u_begin;
+  Task lt;
+  auto load_unit = [&](int st) {
+    if (lu >= u_end) return;
+    const bool starts = lu == seg_end;
+    if (starts) {
+      lt = find_task(args, cum, uniform, lu);
+      seg_end = min(lt.first + lt.units, u_end);
+    }
+    if (lane == 0) {
+      const int t = lu - lt.first;
+      int base, end;
+      const bool own = t >= lt.kr.n_prefix;
+      if (!own) {
+        base = t * SA_KEYS;
+        end = lt.kr.prefix_end;
+      } else if (t < lt.kr.n_sink) {
+        base = (t - lt.kr.n_prefix) * SA_KEYS;
+        end = lt.kr.sink_end;
+      } else {
+        base = lt.kr.lo + (t - lt.kr.n_sink) * SA_KEYS;
+        end = lt.kr.hi;
+      }
+      const void *tk = own ? &args.tmap_k : &args.tmap_pk, *tv = own ? &args.tmap_v : &args.tmap_pv;
+      unsigned char* dst = ring + st * L::STAGE_BYTES;
+      sm100::mbar_arrive_expect_tx(&bars[st], L::STAGE_BYTES);
+#pragma unroll
+      for (int j = 0; j < AC; ++j) sm100::tma_load_4d(dst + j * (SA_KEYS * 128), tk, j * 64, base, lt.hkv, own ? lt.b : 0, &bars[st]);
+#pragma unroll
+      for (int j = 0; j < AC; ++j)
+        sm100::tma_load_4d(dst + L::HALF_BYTES + j * (SA_KEYS * 128), tv, j * 64, base, lt.hkv, own ? lt.b : 0, &bars[st]);
+      heads[st] = UnitHeader{base, end,
+                             (own && !lt.kr.one_position ? 1 : 0) | (starts ? 2 : 0) | (lu + 1 == seg_end ? 4 : 0) |
+                                 (lt.first >= u_begin && lt.first + lt.units <= u_end ? 8 : 0),
+                             lt.b, lt.hkv, lt.mt, lt.len - a.Sq, lt.first};
+    }
+    ++lu;
+  };
+#pragma unroll
+  for (int st = 0; st < SA_STAGES; ++st) load_unit(st);
+  __syncwarp();
+
+  uint4 qf[2][AC][2];
+  float o[AC][8][4];
+  float m[2], l[2];
   int pos[2];
-  uint4 qf[2][KC];
+  int st = 0, phase = 0;
+  for (int u = u_begin; u < u_end; ++u) {
+    const UnitHeader h = heads[st];
+    const uint32_t kbase = sm100::smem_u32(ring + st * L::STAGE_BYTES), vbase = kbase + L::HALF_BYTES;
+    if (h.flags & 2) {
+      const int rows = a.G * a.Sq;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = r_first + g + 8 * h;
-    pos[h] = -1;
-    const bool live = r <= r_last;
-    if (live) pos[h] = off + r / a.G;
+      for (int x = 0; x < 2; ++x) {
+        const int r = h.mt * SA_ROWS + g + 8 * x;
+        const int i = r / a.G, gi = r - i * a.G;
+        pos[x] = r < rows ? h.off + i : -1;
+        const unsigned char* p = static_cast<const unsigned char*>(a.q) +
+                                 (h.b * a.sq.b + static_cast<int64_t>(h.hkv * a.G + gi) * a.sq.h + static_cast<int64_t>(i) * a.sq.s) * 2 + c * 32;
 #pragma unroll
-    for (int j = 0; j < KC; ++j) {
-      qf[h][j] = make_uint4(0, 0, 0, 0);
-      if (live) {
-        const int64_t e = b * a.sq.b + static_cast<int64_t>(hkv * a.G + r % a.G) * a.sq.h + static_cast<int64_t>(r / a.G) * a.sq.s;
-        qf[h][j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + e * 2 + j * 64 + c * 16));
+        for (int j = 0; j < AC; ++j)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            qf[x][j][y] = r < rows ? __ldg(reinterpret_cast<const uint4*>(p + j * 128 + y * 16)) : make_uint4(0, 0, 0, 0);
+        m[x] = -INFINITY;
+        l[x] = 0.0f;
       }
-    }
-  }
-
-  uint4 kf[2][KC], vf[4][VC];
-  // keys beyond the range's end are read from its last key instead and masked
-  auto load_k = [&](const Block& x) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const unsigned char* p = x.k + min(x.base + n * 8 + g, x.end - 1) * x.ks + c * 16;
+      for (int j = 0; j < AC; ++j)
 #pragma unroll
-      for (int j = 0; j < KC; ++j) kf[n][j] = ld_cache16(p + j * 64);
-    }
-  };
-  auto load_v = [&](const Block& x) {
+        for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const unsigned char* p = x.v + min(x.base + (n >> 1) * 8 + 2 * c + (n & 1), x.end - 1) * x.vs + g * 16;
-#pragma unroll
-      for (int j = 0; j < VC; ++j) vf[n][j] = ld_cache16(p + j * 128);
-    }
-  };
-
-  float o[VC][8][4];
-#pragma unroll
-  for (int j = 0; j < VC; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[j][e][i] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
-  // a CTA takes a contiguous share of the blocks, its warps take them in turn
-  const int per = (kr.n_total + cs - 1) / cs;
-  const int t_end = min((rank + 1) * per, kr.n_total);
-  int t = rank * per + warp;
-  const bool one_position = p_first == p_last;   // every live row sees exactly the keys of the ranges
-  Block x;
-  if (t < t_end) {
-    x = block_of(t);
-    load_k(x);
-    load_v(x);
-  }
-  for (; t < t_end; t += SA_WARPS) {
-    const bool more = t + SA_WARPS < t_end;
-    float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-    for (int j = 0; j < KC; ++j)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        mma16816<BF16>(s[n], qf[0][j].x, qf[1][j].x, qf[0][j].y, qf[1][j].y, kf[n][j].x, kf[n][j].y);
-        mma16816<BF16>(s[n], qf[0][j].z, qf[1][j].z, qf[0][j].w, qf[1][j].w, kf[n][j].z, kf[n][j].w);
-      }
-    const Block cur = x;
-    if (more) {
-      x = block_of(t + SA_WARPS);
-      load_k(x);
+          for (int i = 0; i < 4; ++i) o[j][e][i] = 0.0f;
     }
 
-    // scores in log2 units; s[n][2h + e] belongs to row g + 8h and key base + 8n + 2c + e
-    const bool masked = cur.base + SA_KEYS > cur.end || (cur.own && !one_position);
+    if (!sm100::mbar_wait(&bars[st], phase)) {
+      if (lane == 0) sm100::report_timeout(args.status, 60);
+      break;
+    }
+    float s[4][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v = s[n][i] * a.scale_log2;
-        if (masked) {
-          const int key = cur.base + 8 * n + 2 * c + (i & 1), p = pos[i >> 1];
-          if (key >= cur.end || (cur.own && (key > p || (key <= p - a.window && key >= a.sinks)))) v = -INFINITY;
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < AC; ++j)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint4 kf = ld_shared16(kbase + j * (SA_KEYS * 128) + (n * 8 + g) * 128 + (((2 * c + y) ^ g) << 4));
+          mma16816<BF16>(s[n], qf[0][j][y].x, qf[1][j][y].x, qf[0][j][y].y, qf[1][j][y].y, kf.x, kf.y);
+          mma16816<BF16>(s[n], qf[0][j][y].z, qf[1][j][y].z, qf[0][j][y].w, qf[1][j][y].w, kf.z, kf.w);
         }
-        s[n][i] = v;
-      }
+
+    // scores in log2 units; s[n][2x + e] belongs to row g + 8x and key base + 8n + 2c + e
+    const bool own = h.flags & 1, partial = h.base + SA_KEYS > h.end;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] *= a.scale_log2;
+    if (own || partial) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = h.base + 8 * n + 2 * c + (i & 1), p = pos[i >> 1];
+          if (key >= h.end || (own && (key > p || (key <= p - a.window && key >= a.sinks)))) s[n][i] = -INFINITY;
+        }
+    }
     float mx[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+    for (int x = 0; x < 2; ++x) {
+      float v = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
+                      fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
       v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-      mx[h] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+      mx[x] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] + SA_RESCALE || mx[1] > m[1] + SA_RESCALE)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float m_new = fmaxf(m[h], mx[h]);
-        const float f = m[h] == -INFINITY ? 0.0f : ex2(m[h] - m_new);
-        m[h] = m_new;
-        l[h] *= f;
+      for (int x = 0; x < 2; ++x) {
+        const float m_new = fmaxf(m[x], mx[x]);
+        const float f = m[x] == -INFINITY ? 0.0f : ex2(m[x] - m_new);
+        m[x] = m_new;
+        l[x] *= f;
 #pragma unroll
-        for (int j = 0; j < VC; ++j)
+        for (int j = 0; j < AC; ++j)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { o[j][e][2 * h] *= f; o[j][e][2 * h + 1] *= f; }
+          for (int e = 0; e < 8; ++e) { o[j][e][2 * x] *= f; o[j][e][2 * x + 1] *= f; }
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float ref = m[h] == -INFINITY ? 0.0f : m[h];     // nothing seen yet: every weight is exp2(-inf) = 0
+    for (int x = 0; x < 2; ++x) {
+      const float ref = m[x] == -INFINITY ? 0.0f : m[x];     // nothing seen yet: every weight is exp2(-inf) = 0
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float p = ex2(s[n][2 * h + e] - ref);
-          s[n][2 * h + e] = p;
-          l[h] += p;
+          const float p = ex2(s[n][2 * x + e] - ref);
+          s[n][2 * x + e] = p;
+          l[x] += p;
         }
     }
-    const uint32_t pa0 = pack16<BF16>(s[0][0], s[0][1]), pa1 = pack16<BF16>(s[0][2], s[0][3]);
-    const uint32_t pa2 = pack16<BF16>(s[1][0], s[1][1]), pa3 = pack16<BF16>(s[1][2], s[1][3]);
 #pragma unroll
-    for (int j = 0; j < VC; ++j)
+    for (int kk = 0; kk < SA_KEYS / 16; ++kk) {
+      const uint32_t pa0 = pack16<BF16>(s[2 * kk][0], s[2 * kk][1]), pa1 = pack16<BF16>(s[2 * kk][2], s[2 * kk][3]);
+      const uint32_t pa2 = pack16<BF16>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pa3 = pack16<BF16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t v0 = (&vf[0][j].x)[w], v1 = (&vf[1][j].x)[w], v2 = (&vf[2][j].x)[w], v3 = (&vf[3][j].x)[w];
-        mma16816<BF16>(o[j][2 * w], pa0, pa1, pa2, pa3, __byte_perm(v0, v1, 0x5410), __byte_perm(v2, v3, 0x5410));
-        mma16816<BF16>(o[j][2 * w + 1], pa0, pa1, pa2, pa3, __byte_perm(v0, v1, 0x7632), __byte_perm(v2, v3, 0x7632));
+      for (int j = 0; j < AC; ++j) {
+        uint4 vf[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int row = kk * 16 + (n >> 1) * 8 + 2 * c + (n & 1);
+          vf[n] = ld_shared16(vbase + j * (SA_KEYS * 128) + row * 128 + ((g ^ (2 * c + (n & 1))) << 4));
+          // a weight of 0 must not meet what the cache holds behind the range
+          if (partial && h.base + row >= h.end) vf[n] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t v0 = (&vf[0].x)[w], v1 = (&vf[1].x)[w], v2 = (&vf[2].x)[w], v3 = (&vf[3].x)[w];
+          mma16816<BF16>(o[j][2 * w], pa0, pa1, pa2, pa3, __byte_perm(v0, v1, 0x5410), __byte_perm(v2, v3, 0x5410));
+          mma16816<BF16>(o[j][2 * w + 1], pa0, pa1, pa2, pa3, __byte_perm(v0, v1, 0x7632), __byte_perm(v2, v3, 0x7632));
+        }
       }
-    if (more) load_v(x);
-  }
+    }
+    __syncwarp();                                // every lane is done with the stage and its header
+    load_unit(st);
+    __syncwarp();
+    if (++st == SA_STAGES) { st = 0; phase ^= 1; }
 
-  // ---- join the warps: o[j][e][2h + i] is row g + 8h, column 64 j + 8 (2c + i) + e
+    if (h.flags & 4) {
+      // ---- end of a segment: o[j][e][2x + i] is row g + 8x, column 64 j + 8 (2c + i) + e
+      const int rows = min(SA_ROWS, a.G * a.Sq - h.mt * SA_ROWS);
+      const bool whole = h.flags & 8;
+      const int task = (h.b * a.Hkv + h.hkv) * args.m_tiles + h.mt;
+      const int64_t slot = whole ? 2LL * args.n_warps + task : 2LL * share + (h.task_first <= u_begin ? 0 : 1);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (c == 0) { sm_m[warp][g + 8 * h] = m[h]; sm_l[warp][g + 8 * h] = l[h]; }
+      for (int x = 0; x < 2; ++x) {
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+        const int row = g + 8 * x;
+        if (row >= rows) continue;
+        if (whole && !behind_prefix) {
+          const int r = h.mt * SA_ROWS + row, i = r / a.G, gi = r - i * a.G;
+          const float inv = l[x] == 0.0f ? 0.0f : 1.0f / l[x];       // no visible key: 0; NaN passes through
+          const bool sees = pos[x] >= 0;
+          unsigned char* p = static_cast<unsigned char*>(a.out) +
+                             (h.b * a.so.b + static_cast<int64_t>(h.hkv * a.G + gi) * a.so.h + static_cast<int64_t>(i) * a.so.s) * 2 + c * 32;
 #pragma unroll
-    for (int j = 0; j < VC; ++j)
+          for (int j = 0; j < AC; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+            for (int i2 = 0; i2 < 2; ++i2) {
+              uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          *reinterpret_cast<float4*>(&sm_o[warp][g + 8 * h][64 * j + 8 * (2 * c + i) + e]) =
-              make_float4(o[j][e][2 * h + i], o[j][e + 1][2 * h + i], o[j][e + 2][2 * h + i], o[j][e + 3][2 * h + i]);
-  }
-  __syncthreads();
-  if (cs > 1) {
-    // the CTA's own result replaces warp 0's, where the other CTAs of the cluster read it
-    constexpr int PER = SA_ROWS * HD / (SA_WARPS * 32);
-    const int row = threadIdx.x / (HD / PER), d0 = threadIdx.x % (HD / PER) * PER;
-    float mm = sm_m[0][row];
+              for (int e = 0; e < 4; ++e)
+                w[e] = sees ? pack16<BF16>(o[j][2 * e][2 * x + i2] * inv, o[j][2 * e + 1][2 * x + i2] * inv) : 0u;
+              *reinterpret_cast<uint4*>(p + j * 128 + i2 * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else {
+          const int64_t at = slot * args.rows_cap + row;
+          if (c == 0) *reinterpret_cast<float2*>(args.slot_ml + at * 2) = make_float2(m[x], l[x]);
+          float* p = args.slot_o + at * HD + c * 16;
 #pragma unroll
-    for (int w = 1; w < SA_WARPS; ++w) mm = fmaxf(mm, sm_m[w][row]);
-    float f[SA_WARPS], sum = 0.0f;
+          for (int j = 0; j < AC; ++j)
 #pragma unroll
-    for (int w = 0; w < SA_WARPS; ++w) {
-      f[w] = sm_m[w][row] == -INFINITY ? 0.0f : ex2(sm_m[w][row] - mm);
-      sum += f[w] * sm_l[w][row];
-    }
+            for (int i2 = 0; i2 < 2; ++i2)
 #pragma unroll
-    for (int d = 0; d < PER; d += 4) {
-      float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int w = 0; w < SA_WARPS; ++w) {
-        const float4 v = *reinterpret_cast<const float4*>(&sm_o[w][row][d0 + d]);
-        acc.x += f[w] * v.x; acc.y += f[w] * v.y; acc.z += f[w] * v.z; acc.w += f[w] * v.w;
+              for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<float4*>(p + j * 64 + i2 * 8 + e) =
+                    make_float4(o[j][e][2 * x + i2], o[j][e + 1][2 * x + i2], o[j][e + 2][2 * x + i2], o[j][e + 3][2 * x + i2]);
+        }
       }
-      *reinterpret_cast<float4*>(&sm_o[0][row][d0 + d]) = acc;
     }
-    __syncthreads();                             // every reader of the warps' sums is done
-    if (d0 == 0) { sm_m[0][row] = mm; sm_l[0][row] = sum; }
-    sm100::cluster_sync_all();
   }
+  if (behind_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
-  // ---- rows of this CTA: join the parts (warps, or the cluster's CTAs) and the prefix's partial results
-  const int n_parts = cs > 1 ? cs : SA_WARPS;
-  const int rows_here = SA_ROWS / cs, vecs = HD / 8;
-  for (int w = threadIdx.x; w < rows_here * vecs; w += SA_WARPS * 32) {
-    const int row = rank * rows_here + w / vecs, d = w % vecs * 8;
-    const int r = r_first + row;
-    if (r > r_last) continue;
-    const int i = r / a.G, hq = hkv * a.G + r % a.G;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
-    if (off + i >= 0) {
-      auto part_ptr = [&](const float* p, int n) -> const float* {
-        if (cs == 1) return p;
-        return reinterpret_cast<const float*>(__cluster_map_shared_rank(p, n));
-      };
-      const int ws = cs > 1 ? 0 : 1;             // parts are warps of this CTA, or warp slot 0 of every CTA
-      auto pm = [&](int n) { return *part_ptr(&sm_m[ws * n][row], n); };
-      const size_t prow = (static_cast<size_t>(b) * a.Sq + i) * a.G + r % a.G;
-      auto lse_of = [&](int n) { return __ldg(args.part.lse + (static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow); };
-      float mm = -INFINITY;
-      for (int n = 0; n < n_parts; ++n) mm = fmaxf(mm, pm(n));
-      for (int n = 0; n < args.part.splits; ++n) mm = fmaxf(mm, lse_of(n));
-      for (int n = 0; n < n_parts; ++n) {
-        const float mn = pm(n);
-        if (mn == -INFINITY) continue;
-        const float f = ex2(mn - mm);
-        sum += f * *part_ptr(&sm_l[ws * n][row], n);
-        const float* src = part_ptr(&sm_o[ws * n][row][d], n);
+// Adds up the parts of every row that no warp finished alone: `tpr` threads per row, 8 columns each, which take
+// the row's parts in turn (in the order of the keys, then the prefix's).
+constexpr int CA_THREADS = 256;
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_constant__ StreamArgs args, int tpr) {
+  constexpr int VECS = HD / 8;
+  __shared__ float sm_acc[CA_THREADS / 32][VECS][8], sm_ms[CA_THREADS / 32][VECS][2];
+  extern __shared__ int cum[];
+  __shared__ int warp_sum[CA_THREADS / 32];
+  const CacheAttn& a = args.a;
+  // the list of units needs only the lengths, which were there before the first of the kernels started
+  int uniform;
+  const int total = cumulate_units<CA_THREADS>(args, cum, warp_sum, &uniform);
+  const int prefix = args.part.splits == 0 ? a.P : 0;
+  const int rows = a.G * a.Sq;
+  const int64_t row_all = static_cast<int64_t>(blockIdx.x) * (CA_THREADS / tpr) + threadIdx.x / tpr;
+  const int64_t n_rows = static_cast<int64_t>(a.B) * a.Hkv * rows;
+  const bool live = row_all < n_rows;
+  const int r = live ? static_cast<int>(row_all % rows) : 0;
+  const int bh = live ? static_cast<int>(row_all / rows) : 0;
+  const int hkv = bh % a.Hkv, b = bh / a.Hkv;
+  const int i = r / a.G, gi = r - i * a.G;
+  const int mt = r / SA_ROWS, row = r - mt * SA_ROWS;
+  const int t = threadIdx.x % tpr, vec = t % VECS, sub = t / VECS, nsub = tpr / VECS;
+
+  // the task's units, and the shares that hold them
+  const int len = sequence_length(a, b);
+  const int per_head = head_units(a, prefix, len, args.m_tiles);
+  int first;
+  if (uniform) {
+    first = per_head * (b * a.Hkv + hkv);
+  } else {
+    const int e = b / args.group;
+    first = (a.lengths ? cum[e] : 0) + per_head * hkv;
+    for (int x = e * args.group; x < b; ++x) first += head_units(a, prefix, sequence_length(a, x), args.m_tiles) * a.Hkv;
+  }
+  for (int x = 0; x < mt; ++x) first += key_ranges(a, prefix, len, x).n_total;
+  const int units = key_ranges(a, prefix, len, mt).n_total;
+  const Shares shares(total, args.n_warps);
+  int w0 = 0, w1 = -1, first_slot = 0;
+  if (units > 0) {
+    w0 = shares.of(first);
+    w1 = shares.of(first + units - 1);
+    first_slot = first <= shares.begin(w0) ? 0 : 1;        // the later shares start inside the task: their slot 0
+  }
+  const bool behind_prefix = args.part.splits > 0;
+  const bool done = !live || (w0 == w1 && !behind_prefix);       // written by the warp that had it all
+  const bool sees = !done && len - a.Sq + i >= 0;
+  const int task = (b * a.Hkv + hkv) * args.m_tiles + mt;
+
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, mm = -INFINITY;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  auto join = [&](float mn, float ln, float4 u, float4 v) {      // (acc, sum, mm) += a part with maximum mn
+    if (mn == -INFINITY) return;
+    const float m_new = fmaxf(mm, mn);
+    const float f0 = mm == -INFINITY ? 0.0f : ex2(mm - m_new), f1 = ex2(mn - m_new);
+    mm = m_new;
+    sum = f0 * sum + f1 * ln;
+    acc[0] = f0 * acc[0] + f1 * u.x; acc[1] = f0 * acc[1] + f1 * u.y; acc[2] = f0 * acc[2] + f1 * u.z; acc[3] = f0 * acc[3] + f1 * u.w;
+    acc[4] = f0 * acc[4] + f1 * v.x; acc[5] = f0 * acc[5] + f1 * v.y; acc[6] = f0 * acc[6] + f1 * v.z; acc[7] = f0 * acc[7] + f1 * v.w;
+  };
+  if (sees) {
+#pragma unroll 4
+    for (int w = w0 + sub; w <= w1; w += nsub) {
+      const int64_t slot = w0 == w1 ? 2LL * args.n_warps + task : 2LL * w + (w == w0 ? first_slot : 0);
+      const int64_t at = slot * args.rows_cap + row;
+      const float4* src = reinterpret_cast<const float4*>(args.slot_o + at * HD + vec * 8);
+      const float2 ml = *reinterpret_cast<const float2*>(args.slot_ml + at * 2);
+      const float4 u = src[0], v = src[1];
+      join(ml.x, ml.y, u, v);
+    }
+    const size_t prow = (static_cast<size_t>(b) * a.Sq + i) * a.G + gi;
+#pragma unroll 4
+    for (int n = sub; n < args.part.splits; n += nsub) {
+      const size_t e = (static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow;
+      const float4* src = reinterpret_cast<const float4*>(args.part.o + e * HD + vec * 8);
+      const float4 u = src[0], v = src[1];
+      join(args.part.lse[e], 1.0f, u, v);
+    }
+  }
+  // lanes of a warp with the same columns, then the row's warps
+  for (int x = VECS; x < 32; x *= 2) {
+    const float mn = __shfl_xor_sync(0xffffffffu, mm, x), ln = __shfl_xor_sync(0xffffffffu, sum, x);
+    float4 u, v;
+    u.x = __shfl_xor_sync(0xffffffffu, acc[0], x); u.y = __shfl_xor_sync(0xffffffffu, acc[1], x);
+    u.z = __shfl_xor_sync(0xffffffffu, acc[2], x); u.w = __shfl_xor_sync(0xffffffffu, acc[3], x);
+    v.x = __shfl_xor_sync(0xffffffffu, acc[4], x); v.y = __shfl_xor_sync(0xffffffffu, acc[5], x);
+    v.z = __shfl_xor_sync(0xffffffffu, acc[6], x); v.w = __shfl_xor_sync(0xffffffffu, acc[7], x);
+    join(mn, ln, u, v);
+  }
+  if (tpr > 32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane < VECS) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src + e);
-          acc[e] += f * v.x; acc[e + 1] += f * v.y; acc[e + 2] += f * v.z; acc[e + 3] += f * v.w;
-        }
-      }
-      for (int n = 0; n < args.part.splits; ++n) {
-        const float ls = lse_of(n);
-        if (ls == -INFINITY) continue;
-        const float f = ex2(ls - mm);
-        sum += f;
-        const float* src = args.part.o + ((static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow) * HD + d;
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(src + e));
-          acc[e] += f * v.x; acc[e + 1] += f * v.y; acc[e + 2] += f * v.z; acc[e + 3] += f * v.w;
-        }
+      for (int e = 0; e < 8; ++e) sm_acc[warp][lane][e] = acc[e];
+      sm_ms[warp][lane][0] = mm;
+      sm_ms[warp][lane][1] = sum;
+    }
+    __syncthreads();
+    if (sub == 0) {
+      for (int w = warp + 1; w < warp + tpr / 32; ++w) {
+        const float* p = sm_acc[w][vec];
+        join(sm_ms[w][vec][0], sm_ms[w][vec][1], make_float4(p[0], p[1], p[2], p[3]), make_float4(p[4], p[5], p[6], p[7]));
       }
     }
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;     // no visible key: 0; NaN passes through
-    uint32_t out[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = pack16<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    const int64_t e0 = b * a.so.b + hq * a.so.h + static_cast<int64_t>(i) * a.so.s + d;
-    *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + e0 * 2) = make_uint4(out[0], out[1], out[2], out[3]);
   }
-  if (cs > 1) sm100::cluster_sync_all();         // no CTA leaves while another still reads its part
+  if (!done && sub == 0) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;           // no visible key: 0; NaN passes through
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack16<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    const int64_t e0 = b * a.so.b + static_cast<int64_t>(hkv * a.G + gi) * a.so.h + static_cast<int64_t>(i) * a.so.s + vec * 8;
+    *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + e0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // ---------------------------------------------------------------- host side
+struct StreamPlan {
+  int m_tiles, ctas, n_warps, rows_cap, group, groups;
+  int64_t tasks, slots, units;     // units: the most there can be (every sequence at full length)
+};
+
+StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
+  StreamPlan p;
+  const int warps = a.D == 128 ? StreamSmem<128>::WARPS : StreamSmem<64>::WARPS;
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
+  p.m_tiles = static_cast<int>((rows + SA_ROWS - 1) / SA_ROWS);
+  p.rows_cap = static_cast<int>(rows < SA_ROWS ? rows : SA_ROWS);
+  p.tasks = static_cast<int64_t>(a.B) * a.Hkv * p.m_tiles;
+  const int prefix = behind_prefix ? 0 : a.P;
+  int64_t per_head = 0;
+  for (int mt = 0; mt < p.m_tiles; ++mt) per_head += key_ranges(a, prefix, a.Skv, mt).n_total;
+  p.units = per_head * a.B * a.Hkv;
+  // every warp the machine can hold at once, if there is a unit for each
+  const int64_t sms = sm_count();
+  p.ctas = static_cast<int>(p.units < sms ? (p.units < 1 ? 1 : p.units) : sms);
+  p.n_warps = p.ctas * warps;
+  p.group = (a.B + SA_GROUPS - 1) / SA_GROUPS;
+  p.groups = (a.B + p.group - 1) / p.group;
+  p.slots = 2LL * p.n_warps + (behind_prefix ? p.tasks : 0);
+  return p;
+}
+
+size_t stream_bytes(const CacheAttn& a, const StreamPlan& p) {
+  return static_cast<size_t>(p.slots) * p.rows_cap * (a.D + 2) * sizeof(float);
+}
+
 template <int HD, bool BF16>
-int launch_stream_cfg(const StreamArgs& s, int64_t tasks, cudaStream_t stream) {
+int launch_stream_cfg(const StreamArgs& s, int ctas, int tpr, cudaStream_t stream) {
+  using L = StreamSmem<HD>;
   auto kern = stream_attention_kernel<HD, BF16>;
+  constexpr int most = L::FIXED + SA_GROUPS * static_cast<int>(sizeof(int));
+  const size_t table = s.a.lengths ? s.groups * sizeof(int) : 0;
   int dev = 0;
   CDR_CUDA_TRY(cudaGetDevice(&dev));
   static bool configured_dev[64] = {false};
   if (!configured_dev[dev & 63]) {
-    CDR_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    CDR_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     configured_dev[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tasks * s.cluster), 1, 1);
-  cfg.blockDim = dim3(SA_WARPS * 32, 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  cfg.blockDim = dim3(L::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = L::FIXED + table;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(s.cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = 1;
   CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s));
+  const int64_t rows = static_cast<int64_t>(s.a.B) * s.a.Hq * s.a.Sq;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + CA_THREADS / tpr - 1) / (CA_THREADS / tpr)), 1, 1);
+  cfg.blockDim = dim3(CA_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = table;
+  CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, combine_parts_kernel<HD, BF16>, s, tpr));
   return CDR_OK;
 }
 
 }  // namespace
 
-int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, cudaStream_t stream) {
-  StreamArgs s;
+size_t stream_workspace(const CacheAttn& a, bool behind_prefix) { return stream_bytes(a, plan_stream(a, behind_prefix)); }
+
+int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void* ws, cudaStream_t stream) {
+  const StreamPlan p = plan_stream(a, part.splits > 0);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  if (p.units > 0x3fffffff || p.tasks > 0x3fffffff || rows > 0x3fffffff) { set_error("attention: too many row tiles for one launch"); return CDR_ERR_UNSUPPORTED; }
+  StreamArgs s = {};
   s.a = a;
   s.part = part;
-  const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
-  s.m_tiles = static_cast<int>((rows + SA_ROWS - 1) / SA_ROWS);
-  const int64_t tasks = static_cast<int64_t>(a.B) * a.Hkv * s.m_tiles;
-  // Split a task over as many CTAs as keep the machine's 3 resident CTAs per SM busy, as long as every
-  // warp gets two blocks of keys.
-  int64_t keys = a.Skv < static_cast<int64_t>(a.window) + a.sinks + a.Sq ? a.Skv : static_cast<int64_t>(a.window) + a.sinks + a.Sq;
-  if (part.splits == 0) keys += a.P;
-  s.cluster = 1;
-  while (s.cluster < SA_MAX_CLUSTER && tasks * s.cluster < 3 * sm_count() && keys > 2LL * SA_KEYS * SA_WARPS * s.cluster) s.cluster *= 2;
-  if (tasks * s.cluster > 0x7fffffff) { set_error("attention: %lld row tiles are too many for one launch", (long long)tasks); return CDR_ERR_UNSUPPORTED; }
-  if (a.D == 128) return a.bf16 ? launch_stream_cfg<128, true>(s, tasks, stream) : launch_stream_cfg<128, false>(s, tasks, stream);
-  return a.bf16 ? launch_stream_cfg<64, true>(s, tasks, stream) : launch_stream_cfg<64, false>(s, tasks, stream);
+  s.status = device_status_ptr();
+  if (a.Skv > 0) {           // an empty cache, or prefix, is never loaded from
+    if (int rc = make_map(&s.tmap_k, a.k, a, a.Skv, a.Hkv, a.B, a.sk)) return rc;
+    if (int rc = make_map(&s.tmap_v, a.v, a, a.Skv, a.Hkv, a.B, a.sv)) return rc;
+  }
+  if (a.P > 0 && part.splits == 0) {
+    if (int rc = make_map(&s.tmap_pk, a.pk, a, a.P, a.Hkv, 1, a.spk)) return rc;
+    if (int rc = make_map(&s.tmap_pv, a.pv, a, a.P, a.Hkv, 1, a.spv)) return rc;
+  }
+  s.slot_o = static_cast<float*>(ws);
+  s.slot_ml = s.slot_o + p.slots * p.rows_cap * a.D;
+  s.n_warps = p.n_warps;
+  s.m_tiles = p.m_tiles;
+  s.group = p.group;
+  s.groups = p.groups;
+  s.rows_cap = p.rows_cap;
+  // threads per row of the second kernel: by the parts a row may have
+  const int64_t per_task = p.tasks ? p.units / p.tasks : 0, per_warp = p.units / p.n_warps + 1;
+  const int64_t parts = per_task / per_warp + 1 + part.splits;
+  const int tpr = parts <= 4 ? 32 : parts <= 16 ? 64 : 256;
+  if (a.D == 128) return a.bf16 ? launch_stream_cfg<128, true>(s, p.ctas, tpr, stream) : launch_stream_cfg<128, false>(s, p.ctas, tpr, stream);
+  return a.bf16 ? launch_stream_cfg<64, true>(s, p.ctas, tpr, stream) : launch_stream_cfg<64, false>(s, p.ctas, tpr, stream);
 }
 
 // ---------------------------------------------------------------- entry points
@@ -558,11 +850,13 @@ Path choose_path(const CacheAttn& a) {
   return Path::kStream;
 }
 
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
 size_t cache_attention_workspace(const CacheAttn& a) {
   switch (choose_path(a)) {
     case Path::kTile: return kTileCounterBytes;
-    case Path::kPacked: return packed_workspace(a);
-    default: return 0;
+    case Path::kPacked: return round256(packed_workspace(a)) + stream_workspace(a, true);
+    default: return stream_workspace(a, false);
   }
 }
 
@@ -576,9 +870,11 @@ int run_cache_attention(const CacheAttn& a, const char* op, void* ws, size_t ws_
   if (need && !aligned16(ws)) { set_error("%s: workspace must be 16-byte aligned", op); return CDR_ERR_MISALIGNED; }
   PrefixPartials part{nullptr, nullptr, 0, 0};
   if (path == Path::kTile) return launch_tile_attention(a, ws, stream);
-  if (path == Path::kPacked)
+  if (path == Path::kPacked) {
     if (int rc = launch_packed_prefix(a, ws, &part, stream)) return rc;
-  return launch_stream_attention(a, part, stream);
+    ws = static_cast<unsigned char*>(ws) + round256(packed_workspace(a));
+  }
+  return launch_stream_attention(a, part, ws, stream);
 }
 
 }  // namespace

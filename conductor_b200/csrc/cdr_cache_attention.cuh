@@ -43,9 +43,10 @@ struct PrefixPartials {
   int rows;          // B * Sq * G, row (b, i, g) at (b * Sq + i) * G + g
 };
 
-// Few query rows per key head: the keys are streamed once through registers (cdr_cache_attention.cu).
-// part.splits > 0: joined with the partial results; else the prefix is streamed as well.
-int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, cudaStream_t stream);
+// Few query rows per key head: the keys are streamed once (cdr_cache_attention.cu).  part.splits > 0: joined with
+// the partial results (launched right behind the kernel that makes them); else the prefix is streamed as well.
+int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void* ws, cudaStream_t stream);
+size_t stream_workspace(const CacheAttn& a, bool behind_prefix);   // 16-byte aligned start
 
 // Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter.
 constexpr size_t kTileCounterBytes = 256;

@@ -169,8 +169,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;");
+  // dependents start only after everything in front of this kernel is done (the streaming kernel behind the
+  // packed prefix relies on it)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
 
   if (warp < SOFTMAX_WARP0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
   if (warp == 0) {
