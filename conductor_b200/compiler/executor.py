@@ -48,7 +48,7 @@ def make_descriptors(tensors: Sequence[torch.Tensor]):
 _STRIDED_ATTENTION = (Template.WINDOW_ATTENTION, Template.PREFIX_ATTENTION)
 
 
-def _attention_view_ok(t: torch.Tensor) -> bool:
+def attention_view_ok(t: torch.Tensor) -> bool:
     """A view the cache-attention templates read in place: contiguous last dimension, 16-byte aligned
     start, every other stride a positive multiple of 16 bytes (lengths: contiguous)."""
     if t.is_contiguous():
@@ -144,7 +144,7 @@ class GCUKernelExecutor:
         elif launch.template in _STRIDED_ATTENTION:
             if any(t.device != device for t in inputs):
                 raise DeviceError(f"{launch.name}: inputs on different devices")
-            ins = [t if _attention_view_ok(t) else self.make_contiguous(t) for t in inputs]
+            ins = [t if attention_view_ok(t) else self.make_contiguous(t) for t in inputs]
         else:
             ins = [t if t.is_contiguous() else self.make_contiguous(t) for t in inputs]
         if outputs is None:

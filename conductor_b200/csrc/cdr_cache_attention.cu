@@ -56,6 +56,7 @@ struct StreamArgs {
   PrefixPartials part;     // splits > 0: the prefix is already done
   float *slot_o, *slot_ml; // parts: [slot][row of the task][D] and [..][2] = (maximum, sum)
   int n_warps;             // shares
+  int cluster;             // CTAs per task (CLUSTER)
   int m_tiles;             // tasks per (sequence, key head)
   int group, groups;       // sequences per table entry, table entries
   int rows_cap;            // rows of a slot: min(16, G * Sq)
@@ -228,6 +229,40 @@ __device__ __forceinline__ int cumulate_units(const StreamArgs& s, int* cum, int
   return carry;
 }
 
+// 8 columns of an output row as a sum of parts: each part is (maximum, sum of weights, O) in its own reference.
+struct RowSum {
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, top = -INFINITY;
+
+  __device__ __forceinline__ void join(float m, float l, float4 u, float4 v) {
+    if (m == -INFINITY) return;
+    const float m_new = fmaxf(top, m);
+    const float f0 = top == -INFINITY ? 0.0f : ex2(top - m_new), f1 = ex2(m - m_new);
+    top = m_new;
+    sum = f0 * sum + f1 * l;
+    acc[0] = f0 * acc[0] + f1 * u.x; acc[1] = f0 * acc[1] + f1 * u.y; acc[2] = f0 * acc[2] + f1 * u.z; acc[3] = f0 * acc[3] + f1 * u.w;
+    acc[4] = f0 * acc[4] + f1 * v.x; acc[5] = f0 * acc[5] + f1 * v.y; acc[6] = f0 * acc[6] + f1 * v.z; acc[7] = f0 * acc[7] + f1 * v.w;
+  }
+  // with the lane whose number differs in bit x (every lane of the warp calls this)
+  __device__ __forceinline__ void join_lane(int x) {
+    const float m = __shfl_xor_sync(0xffffffffu, top, x), l = __shfl_xor_sync(0xffffffffu, sum, x);
+    float4 u, v;
+    u.x = __shfl_xor_sync(0xffffffffu, acc[0], x); u.y = __shfl_xor_sync(0xffffffffu, acc[1], x);
+    u.z = __shfl_xor_sync(0xffffffffu, acc[2], x); u.w = __shfl_xor_sync(0xffffffffu, acc[3], x);
+    v.x = __shfl_xor_sync(0xffffffffu, acc[4], x); v.y = __shfl_xor_sync(0xffffffffu, acc[5], x);
+    v.z = __shfl_xor_sync(0xffffffffu, acc[6], x); v.w = __shfl_xor_sync(0xffffffffu, acc[7], x);
+    join(m, l, u, v);
+  }
+  template <bool BF16>
+  __device__ __forceinline__ void store(const CacheAttn& a, int b, int hq, int i, int d) const {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;           // no visible key: 0; NaN passes through
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack16<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    const int64_t e0 = b * a.so.b + hq * a.so.h + static_cast<int64_t>(i) * a.so.s + d;
+    *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + e0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
 // what a staged unit is (written with its copies, read when it is used)
 struct __align__(16) UnitHeader {
   int base, end;         // first key; one past the last key that may be used
@@ -248,7 +283,9 @@ struct StreamSmem {
   static constexpr int FIXED = CUM_OFF + 1024;                 // alignment slack
 };
 
-template <int HD, bool BF16>
+// CLUSTER = false: the list in equal shares, parts to scratch.  CLUSTER = true (few tasks): a task belongs to the warps of
+// one thread-block cluster, which add up their parts through distributed shared memory and write the output.
+template <int HD, bool BF16, bool CLUSTER>
 __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_kernel(const __grid_constant__ StreamArgs args) {
   using L = StreamSmem<HD>;
   constexpr int AC = HD / 64;      // 64-column atoms of a row: 128 bytes, 8 pieces
@@ -275,21 +312,35 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
   if (!behind_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 
-  int uniform;
-  const int total = cumulate_units<L::THREADS>(args, cum, warp_sum, &uniform);
-  const Shares shares(total, args.n_warps);
-  const int share = warp * gridDim.x + blockIdx.x;       // neighbouring shares on different SMs
+  int uniform = 0, total, share, n_warps = args.n_warps;
+  const int cs = args.cluster, rank = CLUSTER ? static_cast<int>(blockIdx.x) % cs : 0;
+  Task lt;
+  if constexpr (CLUSTER) {
+    const int task = blockIdx.x / cs;                    // the list is this task's alone
+    lt.mt = task % args.m_tiles;
+    lt.hkv = task / args.m_tiles % a.Hkv;
+    lt.b = task / args.m_tiles / a.Hkv;
+    lt.len = sequence_length(a, lt.b);
+    lt.kr = key_ranges(a, behind_prefix ? 0 : a.P, lt.len, lt.mt);
+    lt.first = 0;
+    lt.units = total = lt.kr.n_total;
+    n_warps = cs * L::WARPS;
+    share = warp * cs + rank;
+  } else {
+    total = cumulate_units<L::THREADS>(args, cum, warp_sum, &uniform);
+    share = warp * gridDim.x + blockIdx.x;               // neighbouring shares on different SMs
+  }
+  const Shares shares(total, n_warps);
   const int u_begin = share < shares.n ? shares.begin(share) : 0;
   const int u_end = share < shares.n ? shares.begin(share + 1) : 0;
 
   // ---- loads run ahead of their use: unit `lu`, in the segment of its task that ends at unit `seg_end`
   int lu = u_begin, seg_end = u_begin;
-  Task lt;
   auto load_unit = [&](int st) {
     if (lu >= u_end) return;
     const bool starts = lu == seg_end;
     if (starts) {
-      lt = find_task(args, cum, uniform, lu);
+      if (!CLUSTER) lt = find_task(args, cum, uniform, lu);
       seg_end = min(lt.first + lt.units, u_end);
     }
     if (lane == 0) {
@@ -327,7 +378,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
 
   uint4 qf[2][AC][2];
   float o[AC][8][4];
-  float m[2], l[2];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   int pos[2];
   int st = 0, phase = 0;
   for (int u = u_begin; u < u_end; ++u) {
@@ -453,7 +504,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
     __syncwarp();
     if (++st == SA_STAGES) { st = 0; phase ^= 1; }
 
-    if (h.flags & 4) {
+    if (!CLUSTER && (h.flags & 4)) {
       // ---- end of a segment: o[j][e][2x + i] is row g + 8x, column 64 j + 8 (2c + i) + e
       const int rows = min(SA_ROWS, a.G * a.Sq - h.mt * SA_ROWS);
       const bool whole = h.flags & 8;
@@ -498,6 +549,71 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
     }
   }
   if (behind_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (CLUSTER) {
+    // ---- every warp's part in its ring (all its units are used), then the live rows' 8-column pieces are shared out over
+    // the CTAs; `tpp` neighbouring threads take the parts of a piece (the cluster's warps, then the prefix's) in turn
+    constexpr int PITCH = HD + 4, VECS = HD / 8;
+    __shared__ float2 sm_ml[L::WARPS][SA_ROWS];
+    float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      const int row = g + 8 * x;
+      if (c == 0) sm_ml[warp][row] = make_float2(m[x], l[x]);
+      if (u_begin < u_end) {
+#pragma unroll
+        for (int j = 0; j < AC; ++j)
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+              *reinterpret_cast<float4*>(part + row * PITCH + c * 16 + j * 64 + i2 * 8 + e) =
+                  make_float4(o[j][e][2 * x + i2], o[j][e + 1][2 * x + i2], o[j][e + 2][2 * x + i2], o[j][e + 3][2 * x + i2]);
+      }
+    }
+    if (cs > 1) sm100::cluster_sync_all(); else __syncthreads();
+    const int rows = a.G * a.Sq, r_first = lt.mt * SA_ROWS, r_live = min(SA_ROWS, rows - r_first);
+    const int pieces = r_live * VECS, per_cta = (pieces + cs - 1) / cs, n_parts = cs * L::WARPS;
+    int tpp = 1;
+    while (tpp < 16 && tpp * 2 * per_cta <= L::THREADS) tpp *= 2;
+    const int sub = threadIdx.x % tpp;
+    const int at_once = L::THREADS / tpp, passes = (per_cta + at_once - 1) / at_once;
+    for (int pass = 0; pass < passes; ++pass) {
+      const int w = pass * at_once + static_cast<int>(threadIdx.x) / tpp;
+      const int piece = rank * per_cta + w;
+      const bool live = w < per_cta && piece < pieces;
+      const int row = live ? piece / VECS : 0, d = live ? piece % VECS * 8 : 0;
+      const int r = r_first + row, i = r / a.G, gi = r - i * a.G;
+      RowSum sum;
+      if (live && lt.len - a.Sq + i >= 0) {
+#pragma unroll 3
+        for (int n = sub; n < n_parts; n += tpp) {
+          const int wn = n % L::WARPS, cn = n / L::WARPS;
+          const float2* pml = &sm_ml[wn][row];
+          const float* po = reinterpret_cast<const float*>(smem + wn * (SA_STAGES * L::STAGE_BYTES)) + row * PITCH + d;
+          if (cs > 1) {
+            pml = static_cast<const float2*>(__cluster_map_shared_rank(pml, cn));
+            po = static_cast<const float*>(__cluster_map_shared_rank(po, cn));
+          }
+          const float2 ml = *pml;
+          const float4 u = reinterpret_cast<const float4*>(po)[0], v = reinterpret_cast<const float4*>(po)[1];
+          sum.join(ml.x, ml.y, u, v);
+        }
+        const size_t prow = (static_cast<size_t>(lt.b) * a.Sq + i) * a.G + gi;
+#pragma unroll 4
+        for (int n = sub; n < args.part.splits; n += tpp) {
+          const size_t e = (static_cast<size_t>(n) * a.Hkv + lt.hkv) * args.part.rows + prow;
+          const float4* src = reinterpret_cast<const float4*>(args.part.o + e * HD + d);
+          const float4 u = src[0], v = src[1];
+          sum.join(args.part.lse[e], 1.0f, u, v);
+        }
+      }
+      for (int x = 1; x < tpp; x *= 2) sum.join_lane(x);
+      if (live && sub == 0) sum.template store<BF16>(a, lt.b, lt.hkv * a.G + gi, i, d);
+    }
+    if (cs > 1) sm100::cluster_sync_all();       // no CTA leaves while another still reads its parts
+  }
 }
 
 // Adds up the parts of every row that no warp finished alone: `tpr` threads per row, 8 columns each, which take
@@ -551,18 +667,9 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
   const bool sees = !done && len - a.Sq + i >= 0;
   const int task = (b * a.Hkv + hkv) * args.m_tiles + mt;
 
-  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, mm = -INFINITY;
+  RowSum sum;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  auto join = [&](float mn, float ln, float4 u, float4 v) {      // (acc, sum, mm) += a part with maximum mn
-    if (mn == -INFINITY) return;
-    const float m_new = fmaxf(mm, mn);
-    const float f0 = mm == -INFINITY ? 0.0f : ex2(mm - m_new), f1 = ex2(mn - m_new);
-    mm = m_new;
-    sum = f0 * sum + f1 * ln;
-    acc[0] = f0 * acc[0] + f1 * u.x; acc[1] = f0 * acc[1] + f1 * u.y; acc[2] = f0 * acc[2] + f1 * u.z; acc[3] = f0 * acc[3] + f1 * u.w;
-    acc[4] = f0 * acc[4] + f1 * v.x; acc[5] = f0 * acc[5] + f1 * v.y; acc[6] = f0 * acc[6] + f1 * v.z; acc[7] = f0 * acc[7] + f1 * v.w;
-  };
   if (sees) {
 #pragma unroll 4
     for (int w = w0 + sub; w <= w1; w += nsub) {
@@ -571,7 +678,7 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
       const float4* src = reinterpret_cast<const float4*>(args.slot_o + at * HD + vec * 8);
       const float2 ml = *reinterpret_cast<const float2*>(args.slot_ml + at * 2);
       const float4 u = src[0], v = src[1];
-      join(ml.x, ml.y, u, v);
+      sum.join(ml.x, ml.y, u, v);
     }
     const size_t prow = (static_cast<size_t>(b) * a.Sq + i) * a.G + gi;
 #pragma unroll 4
@@ -579,48 +686,34 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
       const size_t e = (static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow;
       const float4* src = reinterpret_cast<const float4*>(args.part.o + e * HD + vec * 8);
       const float4 u = src[0], v = src[1];
-      join(args.part.lse[e], 1.0f, u, v);
+      sum.join(args.part.lse[e], 1.0f, u, v);
     }
   }
   // lanes of a warp with the same columns, then the row's warps
-  for (int x = VECS; x < 32; x *= 2) {
-    const float mn = __shfl_xor_sync(0xffffffffu, mm, x), ln = __shfl_xor_sync(0xffffffffu, sum, x);
-    float4 u, v;
-    u.x = __shfl_xor_sync(0xffffffffu, acc[0], x); u.y = __shfl_xor_sync(0xffffffffu, acc[1], x);
-    u.z = __shfl_xor_sync(0xffffffffu, acc[2], x); u.w = __shfl_xor_sync(0xffffffffu, acc[3], x);
-    v.x = __shfl_xor_sync(0xffffffffu, acc[4], x); v.y = __shfl_xor_sync(0xffffffffu, acc[5], x);
-    v.z = __shfl_xor_sync(0xffffffffu, acc[6], x); v.w = __shfl_xor_sync(0xffffffffu, acc[7], x);
-    join(mn, ln, u, v);
-  }
+  for (int x = VECS; x < 32; x *= 2) sum.join_lane(x);
   if (tpr > 32) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane < VECS) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sm_acc[warp][lane][e] = acc[e];
-      sm_ms[warp][lane][0] = mm;
-      sm_ms[warp][lane][1] = sum;
+      for (int e = 0; e < 8; ++e) sm_acc[warp][lane][e] = sum.acc[e];
+      sm_ms[warp][lane][0] = sum.top;
+      sm_ms[warp][lane][1] = sum.sum;
     }
     __syncthreads();
     if (sub == 0) {
       for (int w = warp + 1; w < warp + tpr / 32; ++w) {
         const float* p = sm_acc[w][vec];
-        join(sm_ms[w][vec][0], sm_ms[w][vec][1], make_float4(p[0], p[1], p[2], p[3]), make_float4(p[4], p[5], p[6], p[7]));
+        sum.join(sm_ms[w][vec][0], sm_ms[w][vec][1], make_float4(p[0], p[1], p[2], p[3]), make_float4(p[4], p[5], p[6], p[7]));
       }
     }
   }
-  if (!done && sub == 0) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;           // no visible key: 0; NaN passes through
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack16<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    const int64_t e0 = b * a.so.b + static_cast<int64_t>(hkv * a.G + gi) * a.so.h + static_cast<int64_t>(i) * a.so.s + vec * 8;
-    *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + e0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  if (!done && sub == 0) sum.template store<BF16>(a, b, hkv * a.G + gi, i, vec * 8);
 }
 
 // ---------------------------------------------------------------- host side
 struct StreamPlan {
   int m_tiles, ctas, n_warps, rows_cap, group, groups;
+  int cluster;                     // > 0: a cluster of so many CTAs per task, no scratch
   int64_t tasks, slots, units;     // units: the most there can be (every sequence at full length)
 };
 
@@ -635,13 +728,18 @@ StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
   int64_t per_head = 0;
   for (int mt = 0; mt < p.m_tiles; ++mt) per_head += key_ranges(a, prefix, a.Skv, mt).n_total;
   p.units = per_head * a.B * a.Hkv;
-  // every warp the machine can hold at once, if there is a unit for each
   const int64_t sms = sm_count();
+  p.cluster = 0;
+  if (p.tasks <= sms) {
+    p.cluster = 1;
+    while (p.cluster < 8 && p.tasks * p.cluster * 2 <= sms && per_head > p.m_tiles * p.cluster * warps) p.cluster *= 2;
+  }
+  // every warp the machine can hold at once, if there is a unit for each
   p.ctas = static_cast<int>(p.units < sms ? (p.units < 1 ? 1 : p.units) : sms);
   p.n_warps = p.ctas * warps;
   p.group = (a.B + SA_GROUPS - 1) / SA_GROUPS;
   p.groups = (a.B + p.group - 1) / p.group;
-  p.slots = 2LL * p.n_warps + (behind_prefix ? p.tasks : 0);
+  p.slots = p.cluster ? 0 : 2LL * p.n_warps + (behind_prefix ? p.tasks : 0);
   return p;
 }
 
@@ -650,29 +748,39 @@ size_t stream_bytes(const CacheAttn& a, const StreamPlan& p) {
 }
 
 template <int HD, bool BF16>
-int launch_stream_cfg(const StreamArgs& s, int ctas, int tpr, cudaStream_t stream) {
+int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStream_t stream) {
   using L = StreamSmem<HD>;
-  auto kern = stream_attention_kernel<HD, BF16>;
   constexpr int most = L::FIXED + SA_GROUPS * static_cast<int>(sizeof(int));
-  const size_t table = s.a.lengths ? s.groups * sizeof(int) : 0;
+  const size_t table = s.a.lengths && !p.cluster ? s.groups * sizeof(int) : 0;
   int dev = 0;
   CDR_CUDA_TRY(cudaGetDevice(&dev));
   static bool configured_dev[64] = {false};
   if (!configured_dev[dev & 63]) {
-    CDR_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    CDR_CUDA_TRY(cudaFuncSetAttribute(stream_attention_kernel<HD, BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    CDR_CUDA_TRY(cudaFuncSetAttribute(stream_attention_kernel<HD, BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     configured_dev[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(L::THREADS, 1, 1);
-  cfg.dynamicSmemBytes = L::FIXED + table;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s));
+  cfg.blockDim = dim3(L::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = L::FIXED + table;
+  cfg.stream = stream;
+  if (p.cluster) {
+    cfg.gridDim = dim3(static_cast<unsigned>(p.tasks * p.cluster), 1, 1);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+    CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, stream_attention_kernel<HD, BF16, true>, s));
+    return CDR_OK;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas), 1, 1);
+  CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, stream_attention_kernel<HD, BF16, false>, s));
   const int64_t rows = static_cast<int64_t>(s.a.B) * s.a.Hq * s.a.Sq;
   cfg.gridDim = dim3(static_cast<unsigned>((rows + CA_THREADS / tpr - 1) / (CA_THREADS / tpr)), 1, 1);
   cfg.blockDim = dim3(CA_THREADS, 1, 1);
@@ -704,6 +812,7 @@ int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void
   s.slot_o = static_cast<float*>(ws);
   s.slot_ml = s.slot_o + p.slots * p.rows_cap * a.D;
   s.n_warps = p.n_warps;
+  s.cluster = p.cluster;
   s.m_tiles = p.m_tiles;
   s.group = p.group;
   s.groups = p.groups;
@@ -712,8 +821,8 @@ int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void
   const int64_t per_task = p.tasks ? p.units / p.tasks : 0, per_warp = p.units / p.n_warps + 1;
   const int64_t parts = per_task / per_warp + 1 + part.splits;
   const int tpr = parts <= 4 ? 32 : parts <= 16 ? 64 : 256;
-  if (a.D == 128) return a.bf16 ? launch_stream_cfg<128, true>(s, p.ctas, tpr, stream) : launch_stream_cfg<128, false>(s, p.ctas, tpr, stream);
-  return a.bf16 ? launch_stream_cfg<64, true>(s, p.ctas, tpr, stream) : launch_stream_cfg<64, false>(s, p.ctas, tpr, stream);
+  if (a.D == 128) return a.bf16 ? launch_stream_cfg<128, true>(s, p, tpr, stream) : launch_stream_cfg<128, false>(s, p, tpr, stream);
+  return a.bf16 ? launch_stream_cfg<64, true>(s, p, tpr, stream) : launch_stream_cfg<64, false>(s, p, tpr, stream);
 }
 
 // ---------------------------------------------------------------- entry points

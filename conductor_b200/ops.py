@@ -22,14 +22,18 @@ returns 0.  ``scale`` defaults to ``1 / sqrt(D)``.  The result is contiguous ``[
 """
 from __future__ import annotations
 
+import ctypes
+import operator
 import threading
 from typing import Optional
 
 import torch
 
-from .codegen.kernel_templates import prefix_attention_launch, window_attention_launch
-from .compiler.executor import get_executor
+from .codegen.kernel_templates import CdrLaunchItem, CdrTensor, prefix_attention_launch, window_attention_launch
+from .compiler.executor import attention_view_ok, get_executor, make_descriptors, raise_for_status
+from .compiler.loader import load_library
 from .utils.exceptions import DeviceError, ExecutionError
+from .utils.type_mapping import to_cdr_dtype
 
 __all__ = ["window_attention", "prefix_attention"]
 
@@ -56,52 +60,127 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
 
 
 # ---------------------------------------------------------------- direct calls
-# A launch object keeps its marshalled descriptors, so one is kept per thread, operator and parameter
-# set of recent calls; only data pointers change from call to call.
+# A decode step takes about as long on the GPU as a few Python statements do on the host, so a repeated
+# call (same shapes, strides, types and parameters) only refreshes pointers: its descriptors, parameter
+# block and launch item are kept per thread.  Nothing of the tensors themselves is kept.
 _calls = threading.local()
-_MAX_LAUNCHES = 256
+_MAX_CALLS = 256
 
 
-def _launch_for(key, build):
-    cache = getattr(_calls, "cache", None)
-    if cache is None:
-        cache = _calls.cache = {}
-    launch = cache.get(key)
-    if launch is None:
-        if len(cache) >= _MAX_LAUNCHES:
-            cache.clear()
-        launch = cache[key] = build()
-    return launch
+class _Call:
+    """A marshalled launch: one ``cdr_launch_item`` whose pointers are set before every use."""
+
+    __slots__ = ("name", "item", "address", "inputs", "output", "workspace_bytes", "bytes", "shape", "dtype", "like", "launch_many", "keep")
+
+    def __init__(self, launch, tensors):
+        lib = load_library()
+        out = torch.empty(launch.out_shapes[0], dtype=launch.out_dtypes[0], device="meta")
+        in_desc, out_desc = make_descriptors(tensors), (CdrTensor * 1)()
+        out_desc[0].dtype, out_desc[0].rank = to_cdr_dtype(out.dtype), out.dim()
+        for i, (n, st) in enumerate(zip(out.shape, out.stride())):
+            out_desc[0].shape[i], out_desc[0].stride[i] = n, st
+        params, size = ctypes.cast(ctypes.byref(launch.params), ctypes.c_void_p), ctypes.sizeof(launch.params)
+        need = ctypes.c_size_t(0)
+        out_desc[0].data = tensors[0].data_ptr()      # any valid pointer: only the size is asked for
+        with torch.cuda.device(tensors[0].device):
+            rc = lib.cdr_workspace_bytes(launch.template, in_desc, len(tensors), out_desc, 1, params, size, ctypes.byref(need))
+        raise_for_status(lib, rc, launch.name)
+        self.name, self.workspace_bytes = launch.name, need.value
+        self.shape, self.dtype, self.like = tuple(out.shape), out.dtype, tensors[0].is_contiguous()
+        self.bytes = torch.empty(0, dtype=torch.uint8, device=tensors[0].device)
+        self.launch_many = lib.cdr_launch_many
+        self.inputs, self.output = list(in_desc), out_desc[0]
+        self.item = CdrLaunchItem(launch.template, len(tensors), 1, 0, ctypes.addressof(in_desc), ctypes.addressof(out_desc),
+                                  params.value, size, None, need.value)
+        self.address = ctypes.addressof(self.item)
+        self.keep = (launch, in_desc, out_desc)
+
+    def __call__(self, q, pointers, index):
+        # the output is contiguous; empty_like is the cheaper way to it where q is
+        out = torch.empty_like(q) if self.like else torch.empty(self.shape, dtype=self.dtype, device=q.device)
+        for desc, p in zip(self.inputs, pointers):
+            desc.data = p
+        self.output.data = out.data_ptr()
+        if self.workspace_bytes:
+            # of this call alone: it goes back to the current stream's pool once the launch is enqueued
+            ws = self.bytes.new_empty(self.workspace_bytes)
+            self.item.workspace = ws.data_ptr()
+        if _current_device() == index:
+            rc = self.launch_many(self.address, 1, _raw_stream(index), None)
+        else:
+            with torch.cuda.device(index):
+                rc = self.launch_many(self.address, 1, _raw_stream(index), None)
+        if rc:
+            raise_for_status(load_library(), rc, self.name)
+        return out
 
 
-def _check(name, tensors):
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run(name, build, params, tensors):
+    """Run one of the operators on `tensors`: everything the library's checks depend on is in the key, so a
+    kept call has passed them; only what may change between two such calls is looked at here."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
+                                     "torch.no_grad() or detach the inputs", kernel_name=name)
+    key = (name, params, *[(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+    try:
+        call = _calls.cache.get(key)
+    except AttributeError:
+        _calls.cache, call = {}, None
+    if call is not None:
+        pointers = [t.data_ptr() for t in tensors]
+        low = 0
+        for p in pointers:
+            low |= p
+        if not low & 15:
+            q = tensors[0]
+            return call(q, pointers, q.get_device())
+    return _first_run(name, build, params, tensors, key)
+
+
+def _first_run(name, build, params, tensors, key):
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")
-    needs_grad = False
     for t in tensors:
         if t.device != device:
             raise ExecutionError(f"{name}: tensors on {device} and {t.device}", kernel_name=name)
-        needs_grad |= t.requires_grad
-    if needs_grad and torch.is_grad_enabled():
-        raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
-                             "torch.no_grad() or detach the inputs", kernel_name=name)
+    launch = build(tensors[0], *params)
+    if any(t.data_ptr() % 16 or not attention_view_ok(t) for t in tensors):
+        return get_executor().execute(launch, tensors)[0]      # gathers what cannot be read in place
+    call = _Call(launch, tensors)
+    if len(_calls.cache) >= _MAX_CALLS:
+        _calls.cache.clear()
+    _calls.cache[key] = call
+    return call(tensors[0], [t.data_ptr() for t in tensors], device.index)
+
+
+def _build_window(q, window, sinks, has_lengths, scale):
+    return window_attention_launch("window_attention", q.shape, q.dtype, window, sinks, has_lengths, scale)
+
+
+def _build_prefix(q, has_lengths, scale):
+    return prefix_attention_launch("prefix_attention", q.shape, q.dtype, has_lengths, scale)
 
 
 def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None):
-    tensors = (q, k, v) if lengths is None else (q, k, v, lengths)
-    _check("window_attention", tensors)
-    key = (window, sinks, scale, lengths is None, q.shape, q.dtype, q.stride(), k.shape, k.stride(), v.stride())
-    launch = _launch_for(key, lambda: window_attention_launch("window_attention", q.shape, q.dtype, window, sinks, lengths is not None, scale))
-    return get_executor().execute(launch, tensors)[0]
+    window, sinks, scale = operator.index(window), operator.index(sinks), None if scale is None else float(scale)
+    if lengths is None:
+        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v))
+    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths))
 
 
 def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None):
-    tensors = (q, prefix_k, prefix_v, k, v) if lengths is None else (q, prefix_k, prefix_v, k, v, lengths)
-    _check("prefix_attention", tensors)
-    key = (scale, lengths is None, q.shape, q.dtype, q.stride(), prefix_k.shape, k.shape, k.stride(), v.stride())
-    launch = _launch_for(key, lambda: prefix_attention_launch("prefix_attention", q.shape, q.dtype, lengths is not None, scale))
-    return get_executor().execute(launch, tensors)[0]
+    scale = None if scale is None else float(scale)
+    if lengths is None:
+        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v))
+    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths))
 
 
 # ---------------------------------------------------------------- graph form

@@ -7,7 +7,7 @@ import torch
 import conductor
 from cache_attention_ref import reference
 from conductor.compiler import loader
-from conductor.compiler.executor import _attention_view_ok, make_descriptors
+from conductor.compiler.executor import attention_view_ok, make_descriptors
 from conductor.compiler.jit_compiler import ChoreoJITCompiler
 from conductor.compiler.sharding import batch_inputs
 from conductor.utils.exceptions import ConductorError, DeviceError, UnsupportedOperationError
@@ -131,8 +131,8 @@ def test_arguments_are_checked_by_the_library(built_library):
 
 def test_views_the_kernels_read_in_place():
     base = torch.zeros(2, 9, 4, 64, dtype=torch.bfloat16)
-    assert _attention_view_ok(base) and _attention_view_ok(base.transpose(1, 2)) and _attention_view_ok(base[:, 3:7, 1:2])
-    assert not _attention_view_ok(base.transpose(2, 3)) and not _attention_view_ok(base[:1].expand(2, -1, -1, -1))
-    assert not _attention_view_ok(torch.zeros(2, 9, 4, 67, dtype=torch.bfloat16)[..., :64])
-    assert not _attention_view_ok(torch.zeros(2 * 64 + 1, dtype=torch.bfloat16)[1:].view(1, 1, 2, 64))
-    assert _attention_view_ok(torch.zeros(5, dtype=torch.int32)) and not _attention_view_ok(torch.zeros(10, dtype=torch.int32)[::2])
+    assert attention_view_ok(base) and attention_view_ok(base.transpose(1, 2)) and attention_view_ok(base[:, 3:7, 1:2])
+    assert not attention_view_ok(base.transpose(2, 3)) and not attention_view_ok(base[:1].expand(2, -1, -1, -1))
+    assert not attention_view_ok(torch.zeros(2, 9, 4, 67, dtype=torch.bfloat16)[..., :64])
+    assert not attention_view_ok(torch.zeros(2 * 64 + 1, dtype=torch.bfloat16)[1:].view(1, 1, 2, 64))
+    assert attention_view_ok(torch.zeros(5, dtype=torch.int32)) and not attention_view_ok(torch.zeros(10, dtype=torch.int32)[::2])
