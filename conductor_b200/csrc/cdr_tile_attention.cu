@@ -34,7 +34,7 @@ namespace {
 
 constexpr int HALF = 128, BQ = 256, BKV = 128;    // rows per half, per tile; keys per block
 constexpr int TA_THREADS = 384, SOFTMAX_WARP0 = 4;
-constexpr int REGS_CONTROL = 80, REGS_SOFTMAX = 208;   // 128*80 + 256*208 <= 384*168, the CTA's allocation at launch
+constexpr int REGS_CONTROL = 88, REGS_SOFTMAX = 208;   // 128*80 + 256*208 <= 384*168, the CTA's allocation at launch
 constexpr int TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;   // + 128 * half
 constexpr float kRescale = 8.0f;                  // log2 units
 constexpr int KV_STAGES = 4, TILE_SLOTS = 4, TILE_READERS = 9;
@@ -78,11 +78,15 @@ struct Tile {
   int live[2], fw[2], lw[2]; // the half has rows that see keys; first and last own block of their windows
 
   __device__ __forceinline__ int own_block(int j) const { const int o = j - np; return o < ns ? o : wstart + o - ns; }
-  __device__ __forceinline__ bool active(int h, int j) const {
-    if (!live[h]) return false;
+  // a half with these values has rows that see keys of entry j
+  __device__ __forceinline__ bool active(int half_live, int half_fw, int half_lw, int j) const {
+    if (!half_live) return false;
     if (j < np) return true;
     const int kb = own_block(j);
-    return kb <= lw[h] && (kb < ns || kb >= fw[h]);
+    return kb <= half_lw && (kb < ns || kb >= half_fw);
+  }
+  __device__ __forceinline__ bool active(int h, int j) const {   // h: known to the compiler
+    return active(live[h], fw[h], lw[h], j);
   }
 };
 
@@ -201,6 +205,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         if (k > 0 && !sm100::mbar_wait(&bars[B_QEMPTY], (k - 1) & 1)) { sm100::report_timeout(t.status, 41); break; }
         const int q_bytes = PACKED ? a.Sq * a.G * t.seqs_per_half * HD * 2 : L::TILE_BYTES;
         sm100::mbar_arrive_expect_tx(&bars[B_QFULL], (r.live[0] + r.live[1]) * q_bytes);
+#pragma unroll
         for (int h = 0; h < 2; ++h)
           if (r.live[h])
 #pragma unroll
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         ok = ring_wait(0, 45);
         if (!ok) break;
         sm100::tc_fence_after();
+#pragma unroll
         for (int h = 0; h < 2; ++h)
           if (r.active(h, 0)) issue_s(h, 0);
         ring_free(0);
@@ -300,7 +306,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
             __syncwarp();
           }
         }
-        for (int h = 0; h < 2 && ok; ++h) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!ok) break;
           if (r.active(h, j)) {
             if (!started[h] && tiles_done[h] > 0) {    // the previous tile's epilogue must have read O_h
               ok = wait_all(&bars[B_OFREE + h], (tiles_done[h] - 1) & 1, 47);
@@ -366,11 +374,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const int row0 = r.q0 + g * HALF;
       const int p_first = r.off + row0, p_last = r.off + min(row0 + HALF, a.Sq) - 1;
       const int pos = p_first + row_in_half;         // this row's position (PACKED: unused)
+      // (selected, not indexed: an index that the compiler does not know would put the tile into local memory)
+      const int live = g ? r.live[1] : r.live[0], fw = g ? r.fw[1] : r.fw[0], lw = g ? r.lw[1] : r.lw[0];
       float m_ref = -INFINITY, l0 = 0.0f, l1 = 0.0f;
       bool first = true;
 
       for (int j = 0; j < r.n_iter; ++j) {
-        if (!r.active(g, j)) continue;
+        if (!r.active(live, fw, lw, j)) continue;
         if (!sm100::mbar_wait(&bars[B_SFULL + g], n & 1)) { sm100::report_timeout(t.status, 52); ok = false; break; }
         ++n;
         sm100::tc_fence_after();
@@ -399,12 +409,21 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
                 if (c * 32 + i > see) sr[c][i] = __float_as_uint(-INFINITY);
           }
           if (key0 <= p_last - a.window && key0 + BKV > a.sinks) {   // keys in front of some row's window
-            const int gone = pos - a.window - key0, sink = a.sinks - key0;   // hidden: i <= gone and i >= sink
+            const int gone = pos - a.window - key0;  // hidden: i <= gone, unless among the sinks
+            if (key0 >= a.sinks) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c * 32 + i <= gone && c * 32 + i >= sink) sr[c][i] = __float_as_uint(-INFINITY);
+                for (int i = 0; i < 32; ++i)
+                  if (c * 32 + i <= gone) sr[c][i] = __float_as_uint(-INFINITY);
+            } else {
+              const int sink = a.sinks - key0;
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (c * 32 + i <= gone && c * 32 + i >= sink) sr[c][i] = __float_as_uint(-INFINITY);
+            }
           }
         }
 
@@ -454,11 +473,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       if (!ok) break;
 
       // ---- epilogue: O / l; O_h is handed back after the last read
-      if (!r.live[g] && (PACKED || row0 >= a.Sq)) continue;
+      if (!live && (PACKED || row0 >= a.Sq)) continue;
       const float l = l0 + l1;
-      const bool none = !r.live[g] || (!PACKED && pos < 0) || l == 0.0f;
+      const bool none = !live || (!PACKED && pos < 0) || l == 0.0f;
       const float inv = 1.0f / l;
-      if (r.live[g]) {
+      if (live) {
         if (!sm100::mbar_wait(&bars[B_PVDONE + g], (n - 1) & 1)) { sm100::report_timeout(t.status, 53); ok = false; break; }
         sm100::tc_fence_after();
       }
@@ -492,7 +511,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t w[16];
-          if (r.live[g]) {
+          if (live) {
             uint32_t o[32];
             sm100::tmem_ld32(o_taddr + c * 32, o);
             sm100::tmem_ld_wait();
