@@ -37,6 +37,7 @@ constexpr int TA_THREADS = 384, SOFTMAX_WARP0 = 4;
 constexpr int REGS_CONTROL = 88, REGS_SOFTMAX = 208;   // 128*80 + 256*208 <= 384*168, the CTA's allocation at launch
 constexpr int TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;   // + 128 * half
 constexpr float kRescale = 8.0f;                  // log2 units
+constexpr int SINK_COLS = 32;                     // a block of sinks alone is cut to so many keys
 constexpr int KV_STAGES = 4, TILE_SLOTS = 4, TILE_READERS = 9;
 
 struct TileArgs {
@@ -76,6 +77,7 @@ struct Tile {
   int ns, wstart;            // own blocks: [0, ns) and [wstart, ...)
   int n_iter;
   int live[2], fw[2], lw[2]; // the half has rows that see keys; first and last own block of their windows
+  int light[2];              // entry 0 holds nothing but at most 32 sinks for the half
 
   __device__ __forceinline__ int own_block(int j) const { const int o = j - np; return o < ns ? o : wstart + o - ns; }
   // a half with these values has rows that see keys of entry j
@@ -89,6 +91,31 @@ struct Tile {
     return active(live[h], fw[h], lw[h], j);
   }
 };
+
+// The first block of a tile when it is sinks alone: `see` of its 32 columns are visible to this row.
+template <bool BF16>
+__device__ __forceinline__ void softmax_sinks(int see, float scale_log2, uint32_t s_taddr, float& m_ref, float& l) {
+  uint32_t sr[SINK_COLS], pw[SINK_COLS / 2];
+  sm100::tmem_ld32(s_taddr, sr);
+  sm100::tmem_ld_wait();
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SINK_COLS; ++i) {
+    if (i >= see) sr[i] = __float_as_uint(-INFINITY);
+    top = fmaxf(top, __uint_as_float(sr[i]));
+  }
+  m_ref = top * scale_log2;
+  const float neg_m = m_ref == -INFINITY ? 0.0f : -m_ref;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < SINK_COLS; i += 2) {
+    const float p0 = fast_exp2(fmaf(__uint_as_float(sr[i]), scale_log2, neg_m)), p1 = fast_exp2(fmaf(__uint_as_float(sr[i + 1]), scale_log2, neg_m));
+    sum += p0 + p1;
+    pw[i / 2] = pack_pair<BF16>(p0, p1);
+  }
+  l = sum;
+  sm100::tmem_st16(s_taddr, pw);
+}
 
 template <bool PACKED>
 __device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len, Tile& r) {
@@ -105,7 +132,7 @@ __device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len,
     const int np = (a.P + BKV - 1) / BKV;
     r.p0 = split * t.split_blocks;
     r.np = min(t.split_blocks, np - r.p0);
-    r.ns = r.wstart = 0;
+    r.ns = r.wstart = r.light[0] = r.light[1] = 0;
     r.n_iter = r.np;
     r.live[0] = 1;
     r.live[1] = r.b + t.seqs_per_half < a.B;
@@ -133,9 +160,12 @@ __device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len,
     r.lw[h] = last / BKV;
     if (r.live[h]) { wlo = min(wlo, r.fw[h]); whi = max(whi, r.lw[h]); p_max = max(p_max, last); }
   }
-  r.p0 = r.np = r.ns = r.wstart = r.n_iter = 0;
+  r.p0 = r.np = r.ns = r.wstart = r.n_iter = r.light[0] = r.light[1] = 0;
   if (p_max >= 0) {
     r.np = (a.P + BKV - 1) / BKV;
+    const bool few = r.np == 0 && a.sinks > 0 && a.sinks <= SINK_COLS;
+    r.light[0] = few && r.live[0] && r.fw[0] > 0;
+    r.light[1] = few && r.live[1] && r.fw[1] > 0;
     r.ns = (min(a.sinks, p_max + 1) + BKV - 1) / BKV;
     r.wstart = max(r.ns, wlo);
     r.n_iter = r.np + r.ns + max(whi - r.wstart + 1, 0);
@@ -232,6 +262,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
     // ------------------------------------------------------------ MMA issuer (convergent warp, elected lane)
     const bool leader = sm100::elect_one();
     constexpr uint32_t idesc_s = sm100::umma_idesc_f16(HALF, BKV, BF16, false, false);
+    constexpr uint32_t idesc_light = sm100::umma_idesc_f16(HALF, SINK_COLS, BF16, false, false);
     constexpr uint32_t idesc_o = sm100::umma_idesc_f16(HALF, HD, BF16, false, true);  // V is MN-major
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
       const bool done = __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity));
@@ -261,7 +292,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       if (!ok) break;
       auto ring_wait = [&](int i, int site) { const int n = ring + i; return wait_all(&bars[B_FULL + n % KV_STAGES], (n / KV_STAGES) & 1, site); };
       auto ring_free = [&](int i) { commit(&bars[B_EMPTY + (ring + i) % KV_STAGES]); };
-      auto issue_s = [&](int h, int j) {
+      auto issue_s = [&](int h, int j, uint32_t idesc) {
         const uint32_t q_addr = sm100::smem_u32(smem + L::Q_OFF + h * L::TILE_BYTES);
         const uint32_t k_addr = sm100::smem_u32(smem + L::KV_OFF + ((ring + 2 * j) % KV_STAGES) * L::TILE_BYTES);
         const uint32_t d = tmem_base + TMEM_S + h * 128;
@@ -269,7 +300,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t o = (kk / 4) * (128 * 128) + (kk % 4) * 32;
-            sm100::umma_f16_ss(d, sm100::umma_desc_k_sw128(q_addr + o), sm100::umma_desc_k_sw128(k_addr + o), idesc_s, kk > 0 ? 1u : 0u);
+            sm100::umma_f16_ss(d, sm100::umma_desc_k_sw128(q_addr + o), sm100::umma_desc_k_sw128(k_addr + o), idesc, kk > 0 ? 1u : 0u);
           }
           sm100::umma_commit(&bars[B_SFULL + h]);
         }
@@ -282,7 +313,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         sm100::tc_fence_after();
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (r.active(h, 0)) issue_s(h, 0);
+          if (r.active(h, 0)) {
+            if (!PACKED && r.light[h]) issue_s(h, 0, idesc_light);
+            else issue_s(h, 0, idesc_s);
+          }
         ring_free(0);
       }
       if (n_iter <= 1) commit(&bars[B_QEMPTY]);
@@ -321,10 +355,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
             const uint32_t p_tmem = tmem_base + TMEM_S + h * 128;
             if (leader) {
               const uint32_t acc = started[h] ? 1u : 0u;
+              auto products = [&](int steps) {
 #pragma unroll
-              for (int kk = 0; kk < BKV / 16; ++kk)
-                sm100::umma_f16_ts(tmem_base + TMEM_O + h * 128, p_tmem + kk * 8, sm100::umma_desc_mn_sw128(v_addr + kk * (16 * 128), 128 * 128),
-                                   idesc_o, kk > 0 ? 1u : acc);
+                for (int kk = 0; kk < steps; ++kk)
+                  sm100::umma_f16_ts(tmem_base + TMEM_O + h * 128, p_tmem + kk * 8, sm100::umma_desc_mn_sw128(v_addr + kk * (16 * 128), 128 * 128),
+                                     idesc_o, kk > 0 ? 1u : acc);
+              };
+              if (!PACKED && j == 0 && r.light[h]) products(SINK_COLS / 16);
+              else products(BKV / 16);
               sm100::umma_commit(&bars[B_PVDONE + h]);
             }
             __syncwarp();
@@ -337,7 +375,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
               k_ready = true;
               sm100::tc_fence_after();
             }
-            issue_s(h, j + 1);
+            issue_s(h, j + 1, idesc_s);
           }
         }
         if (!ok) break;
@@ -375,7 +413,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const int p_first = r.off + row0, p_last = r.off + min(row0 + HALF, a.Sq) - 1;
       const int pos = p_first + row_in_half;         // this row's position (PACKED: unused)
       // (selected, not indexed: an index that the compiler does not know would put the tile into local memory)
-      const int live = g ? r.live[1] : r.live[0], fw = g ? r.fw[1] : r.fw[0], lw = g ? r.lw[1] : r.lw[0];
+      const int live = g ? r.live[1] : r.live[0], fw = g ? r.fw[1] : r.fw[0], lw = g ? r.lw[1] : r.lw[0],
+                light = g ? r.light[1] : r.light[0];
       float m_ref = -INFINITY, l0 = 0.0f, l1 = 0.0f;
       bool first = true;
 
@@ -384,6 +423,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         if (!sm100::mbar_wait(&bars[B_SFULL + g], n & 1)) { sm100::report_timeout(t.status, 52); ok = false; break; }
         ++n;
         sm100::tc_fence_after();
+        if (!PACKED && j == 0 && light) {
+          // sinks alone: 32 columns of scores, of which this row sees those in front of min(sinks, its position)
+          first = false;
+          softmax_sinks<BF16>(min(a.sinks, pos + 1), a.scale_log2, s_taddr, m_ref, l0);
+          sm100::tmem_st_wait();
+          sm100::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&bars[B_PFULL + g]);
+          continue;
+        }
         uint32_t sr[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) sm100::tmem_ld32(s_taddr + c * 32, sr[c]);
