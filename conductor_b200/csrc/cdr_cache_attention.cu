@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
           const float4 u = reinterpret_cast<const float4*>(po)[0], v = reinterpret_cast<const float4*>(po)[1];
           sum.join(ml.x, ml.y, u, v);
         }
-        const size_t prow = (static_cast<size_t>(lt.b) * a.Sq + i) * a.G + gi;
+        const int prow = args.part.splits ? args.part.row_of(a, lt.b, i, gi) : 0;
 #pragma unroll 4
         for (int n = sub; n < args.part.splits; n += tpp) {
           const size_t e = (static_cast<size_t>(n) * a.Hkv + lt.hkv) * args.part.rows + prow;
@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
       const float4 u = src[0], v = src[1];
       sum.join(ml.x, ml.y, u, v);
     }
-    const size_t prow = (static_cast<size_t>(b) * a.Sq + i) * a.G + gi;
+    const int prow = behind_prefix ? args.part.row_of(a, b, i, gi) : 0;
 #pragma unroll 4
     for (int n = sub; n < args.part.splits; n += nsub) {
       const size_t e = (static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow;
@@ -728,7 +728,8 @@ StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
   int64_t per_head = 0;
   for (int mt = 0; mt < p.m_tiles; ++mt) per_head += key_ranges(a, prefix, a.Skv, mt).n_total;
   p.units = per_head * a.B * a.Hkv;
-  const int64_t sms = sm_count();
+  // (behind the packed product: on the SMs that it leaves)
+  const int64_t sms = behind_prefix ? (sm_count() > packed_ctas(a) ? sm_count() - packed_ctas(a) : 1) : sm_count();
   p.cluster = 0;
   if (p.tasks <= sms) {
     p.cluster = 1;
@@ -790,6 +791,8 @@ int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStr
 }
 
 }  // namespace
+
+float stream_units(const CacheAttn& a) { return static_cast<float>(a.B) * a.Hkv * head_units(a, 0, a.Skv, static_cast<int>((static_cast<int64_t>(a.G) * a.Sq + SA_ROWS - 1) / SA_ROWS)); }
 
 size_t stream_workspace(const CacheAttn& a, bool behind_prefix) { return stream_bytes(a, plan_stream(a, behind_prefix)); }
 
@@ -976,8 +979,8 @@ int run_cache_attention(const CacheAttn& a, const char* op, void* ws, size_t ws_
     set_error("%s: workspace of %zu bytes required, got %zu", op, need, ws ? ws_bytes : (size_t)0);
     return CDR_ERR_WORKSPACE;
   }
-  if (need && !aligned16(ws)) { set_error("%s: workspace must be 16-byte aligned", op); return CDR_ERR_MISALIGNED; }
-  PrefixPartials part{nullptr, nullptr, 0, 0};
+  if (need && (reinterpret_cast<uintptr_t>(ws) & 31u)) { set_error("%s: workspace must be 32-byte aligned", op); return CDR_ERR_MISALIGNED; }
+  PrefixPartials part{nullptr, nullptr, 0, 0, 1};
   if (path == Path::kTile) return launch_tile_attention(a, ws, stream);
   if (path == Path::kPacked) {
     if (int rc = launch_packed_prefix(a, ws, &part, stream)) return rc;

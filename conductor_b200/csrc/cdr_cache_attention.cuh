@@ -37,16 +37,24 @@ struct CacheAttn {
 // Partial results of the shared prefix, one per key split and packed query row, in caller scratch:
 // O already divided by its sum, and log2 of the sum of exponentials (base 2, scaled scores).
 struct PrefixPartials {
-  const float* o;    // [splits][Hkv][rows][D]
-  const float* lse;  // [splits][Hkv][rows]
-  int splits;        // 0: none
-  int rows;          // B * Sq * G, row (b, i, g) at (b * Sq + i) * G + g
+  const float* o;      // [splits][Hkv][rows][D]
+  const float* lse;    // [splits][Hkv][rows]
+  int splits;          // 0: none
+  int rows;            // packed rows: 128 per group of `seqs` sequences
+  int seqs;
+
+  // row of query i, head gi of its group, sequence b; its part n is at (n * Hkv + hkv) * rows + row
+  __host__ __device__ __forceinline__ int row_of(const CacheAttn& a, int b, int i, int gi) const {
+    const int group = b / seqs;
+    return group * 128 + ((b - group * seqs) * a.G + gi) * a.Sq + i;
+  }
 };
 
 // Few query rows per key head: the keys are streamed once (cdr_cache_attention.cu).  part.splits > 0: joined with
 // the partial results (launched right behind the kernel that makes them); else the prefix is streamed as well.
 int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void* ws, cudaStream_t stream);
 size_t stream_workspace(const CacheAttn& a, bool behind_prefix);   // 16-byte aligned start
+float stream_units(const CacheAttn& a);        // 16 KB (D = 128) pieces of own keys, at full lengths
 
 // Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter.
 constexpr size_t kTileCounterBytes = 256;
@@ -54,7 +62,8 @@ constexpr size_t kTileCounterBytes = 256;
 int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream);
 // the shared prefix alone, for G * Sq <= 128 query rows per sequence and key head, into *part in `ws`
 int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream);
-size_t packed_workspace(const CacheAttn& a);   // with the counter; 16-byte aligned start
+size_t packed_workspace(const CacheAttn& a);   // with the counter; 32-byte aligned start
+int packed_ctas(const CacheAttn& a);           // SMs it takes; the streaming kernel behind it runs on the others
 
 #ifdef __CUDACC__
 __device__ __forceinline__ int sequence_length(const CacheAttn& a, int b) {

@@ -19,6 +19,7 @@
 //     scratch in fp32, where the streaming kernel joins them with the sequences' own keys.
 #include <cuda.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include "cdr_attention_softmax.cuh"
 #include "cdr_cache_attention.cuh"
@@ -59,8 +60,10 @@ struct TileSmem {
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int BAR_OFF = KV_OFF + KV_STAGES * TILE_BYTES;
   static constexpr int STAGE_OFF = BAR_OFF + 256;
-  static constexpr int STAGE_BYTES = 8 * 32 * 64;
+  static constexpr int STAGE_BYTES = 8 * 32 * 64;              // 8 softmax warps x 32 rows x 32 16-bit columns
+  static constexpr int PART_STAGE_BYTES = 2 * STAGE_BYTES;     // PACKED: fp32 columns
   static constexpr size_t TOTAL = STAGE_OFF + STAGE_BYTES + 1024;
+  static constexpr size_t TOTAL_PACKED = STAGE_OFF + PART_STAGE_BYTES + 1024;
 };
 
 enum { B_QFULL = 0, B_QEMPTY = 1, B_FULL = 2, B_EMPTY = B_FULL + KV_STAGES, B_SFULL = B_EMPTY + KV_STAGES, B_PFULL = B_SFULL + 2,
@@ -231,7 +234,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         if (!valid) break;
         Tile r;
         decode_tile<PACKED>(t, idx, len, r);
-        idx = t.next_tile ? static_cast<int>(gridDim.x + atomicAdd(t.next_tile, 1u)) : t.total_tiles;
+        // packed tiles are alike and taken in turn; the others go to whoever is free
+        idx = PACKED ? idx + static_cast<int>(gridDim.x) : t.next_tile ? static_cast<int>(gridDim.x + atomicAdd(t.next_tile, 1u)) : t.total_tiles;
         if (k > 0 && !sm100::mbar_wait(&bars[B_QEMPTY], (k - 1) & 1)) { sm100::report_timeout(t.status, 41); break; }
         const int q_bytes = PACKED ? a.Sq * a.G * t.seqs_per_half * HD * 2 : L::TILE_BYTES;
         sm100::mbar_arrive_expect_tx(&bars[B_QFULL], (r.live[0] + r.live[1]) * q_bytes);
@@ -281,7 +285,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const int slot = k % TILE_SLOTS;
       ok = wait_all(&bars[B_TFULL + slot], (k / TILE_SLOTS) & 1, 43);
       if (!ok) break;
-      const int idx = tile_ring[2 * slot], len = tile_ring[2 * slot + 1];
+      // the reduction tells the compiler that all lanes hold the same tile: what follows from it (ring positions, operand
+      // descriptors) then lives in uniform registers, where tcgen05.mma reads it
+      const int idx = __reduce_max_sync(0xffffffffu, tile_ring[2 * slot]), len = __reduce_max_sync(0xffffffffu, tile_ring[2 * slot + 1]);
       __syncwarp();
       if (leader) sm100::mbar_arrive(&bars[B_TEMPTY + slot]);
       if (idx < 0) break;
@@ -296,11 +302,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         const uint32_t q_addr = sm100::smem_u32(smem + L::Q_OFF + h * L::TILE_BYTES);
         const uint32_t k_addr = sm100::smem_u32(smem + L::KV_OFF + ((ring + 2 * j) % KV_STAGES) * L::TILE_BYTES);
         const uint32_t d = tmem_base + TMEM_S + h * 128;
+        const uint64_t qd = sm100::umma_desc_k_sw128(q_addr), kd = sm100::umma_desc_k_sw128(k_addr);
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t o = (kk / 4) * (128 * 128) + (kk % 4) * 32;
-            sm100::umma_f16_ss(d, sm100::umma_desc_k_sw128(q_addr + o), sm100::umma_desc_k_sw128(k_addr + o), idesc, kk > 0 ? 1u : 0u);
+            const uint32_t o = ((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4;      // the address field counts 16 bytes
+            sm100::umma_f16_ss(d, qd + o, kd + o, idesc, kk > 0 ? 1u : 0u);
           }
           sm100::umma_commit(&bars[B_SFULL + h]);
         }
@@ -355,11 +362,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
             const uint32_t p_tmem = tmem_base + TMEM_S + h * 128;
             if (leader) {
               const uint32_t acc = started[h] ? 1u : 0u;
+              const uint64_t vd = sm100::umma_desc_mn_sw128(v_addr, 128 * 128);
               auto products = [&](int steps) {
 #pragma unroll
                 for (int kk = 0; kk < steps; ++kk)
-                  sm100::umma_f16_ts(tmem_base + TMEM_O + h * 128, p_tmem + kk * 8, sm100::umma_desc_mn_sw128(v_addr + kk * (16 * 128), 128 * 128),
-                                     idesc_o, kk > 0 ? 1u : acc);
+                  sm100::umma_f16_ts(tmem_base + TMEM_O + h * 128, p_tmem + kk * 8, vd + kk * ((16 * 128) >> 4), idesc_o, kk > 0 ? 1u : acc);
               };
               if (!PACKED && j == 0 && r.light[h]) products(SINK_COLS / 16);
               else products(BKV / 16);
@@ -531,12 +538,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         sm100::tc_fence_after();
       }
       if constexpr (PACKED) {
-        const int per_seq = a.G * a.Sq, bb = row_in_half / per_seq, rem = row_in_half - bb * per_seq;
-        const int b = r.b + g * t.seqs_per_half + bb;
-        const bool write = bb < t.seqs_per_half && b < a.B;
-        const size_t prow = (static_cast<size_t>(b) * a.Sq + rem % a.Sq) * a.G + rem / a.Sq;
-        const size_t at = (static_cast<size_t>(r.off) * a.Hkv + r.hkv) * t.part_rows + prow;
-        if (write) t.part_lse[at] = none ? -INFINITY : m_ref + __log2f(l);
+        // rows in packed order; 32 columns at a time through shared memory (16-byte pieces of a row XORed with the
+        // row), so that four rows of 128 contiguous bytes leave with one instruction: a store per lane of its own
+        // row touches 32 lines and took 10000 cycles per tile
+        const int half_rows = a.G * a.Sq * t.seqs_per_half;
+        const int64_t at = (static_cast<int64_t>(r.off) * a.Hkv + r.hkv) * t.part_rows + (r.b / t.seqs_per_half + g) * HALF;
+        if (row_in_half < half_rows) t.part_lse[at + row_in_half] = none ? -INFINITY : m_ref + __log2f(l);
+        unsigned char* part_stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * (32 * 128);
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
@@ -547,13 +555,18 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&bars[B_OFREE + g]);
           }
-          if (write) {
-            float4* dst = reinterpret_cast<float4*>(t.part_o + at * HD + c * 32);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = none ? make_float4(0, 0, 0, 0)
-                            : make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                          __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+          for (int i = 0; i < 32; ++i) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+          __syncwarp();                              // the stage has been read
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(part_stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3), piece = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4*>(part_stage + row * 128 + ((piece ^ (row & 7)) << 4));
+            if (q * 32 + row < half_rows) *reinterpret_cast<uint4*>(t.part_o + (at + q * 32 + row) * HD + c * 32 + piece * 4) = v;
           }
         }
       } else {
@@ -603,9 +616,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 
 // ---------------------------------------------------------------- host side
 template <int HD, bool BF16, bool PACKED>
-int launch_tile_cfg(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stream) {
+int launch_tile_cfg(TileArgs& t, int64_t tiles, int ctas, void* counter, cudaStream_t stream) {
   auto kern = tile_attention_kernel<HD, BF16, PACKED>;
-  constexpr size_t smem = TileSmem<HD>::TOTAL;
+  constexpr size_t smem = PACKED ? TileSmem<HD>::TOTAL_PACKED : TileSmem<HD>::TOTAL;
   static bool configured_dev[64] = {false};
   int dev = 0;
   CDR_CUDA_TRY(cudaGetDevice(&dev));
@@ -622,10 +635,9 @@ int launch_tile_cfg(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stre
   }
   t.total_tiles = static_cast<int>(tiles);
   t.status = device_status_ptr();
-  const int64_t sms = sm_count();
-  const int64_t grid = tiles < sms ? tiles : sms;
+  const int64_t grid = tiles < ctas ? tiles : ctas;
   t.next_tile = nullptr;
-  if (tiles > grid) {            // CTAs draw tiles beyond their first from a counter
+  if (!PACKED && tiles > grid) { // CTAs draw tiles beyond their first from a counter
     t.next_tile = static_cast<unsigned int*>(counter);
     CDR_CUDA_TRY(cudaMemsetAsync(t.next_tile, 0, sizeof(unsigned int), stream));
   }
@@ -644,10 +656,10 @@ int launch_tile_cfg(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stre
 }
 
 template <bool PACKED>
-int launch_tile_typed(TileArgs& t, int64_t tiles, void* counter, cudaStream_t stream) {
+int launch_tile_typed(TileArgs& t, int64_t tiles, int ctas, void* counter, cudaStream_t stream) {
   if (tiles > 0x3fffffff) { set_error("attention: too many tiles"); return CDR_ERR_UNSUPPORTED; }
-  if (t.a.D == 128) return t.a.bf16 ? launch_tile_cfg<128, true, PACKED>(t, tiles, counter, stream) : launch_tile_cfg<128, false, PACKED>(t, tiles, counter, stream);
-  return t.a.bf16 ? launch_tile_cfg<64, true, PACKED>(t, tiles, counter, stream) : launch_tile_cfg<64, false, PACKED>(t, tiles, counter, stream);
+  if (t.a.D == 128) return t.a.bf16 ? launch_tile_cfg<128, true, PACKED>(t, tiles, ctas, counter, stream) : launch_tile_cfg<128, false, PACKED>(t, tiles, ctas, counter, stream);
+  return t.a.bf16 ? launch_tile_cfg<64, true, PACKED>(t, tiles, ctas, counter, stream) : launch_tile_cfg<64, false, PACKED>(t, tiles, ctas, counter, stream);
 }
 
 int map_heads(CUtensorMap* m, const void* base, const CacheAttn& a, int64_t S, int64_t H, int64_t B, const HeadStrides& st, int box_d,
@@ -683,42 +695,81 @@ int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
   if (BH * t.n_qtiles > 0x3fffffff) { set_error("attention: too many tiles"); return CDR_ERR_UNSUPPORTED; }
   const int fill = sm_count() / t.n_qtiles;
   t.group_heads = static_cast<int>(fill < 1 ? 1 : fill > BH ? BH : fill);
-  return launch_tile_typed<false>(t, BH * t.n_qtiles, ws, stream);
+  return launch_tile_typed<false>(t, BH * t.n_qtiles, sm_count(), ws, stream);
 }
 
-// How the shared prefix is cut for the packed product: sequences per half, row tiles, key splits.
-void plan_packed(const CacheAttn& a, int* seqs_per_half, int* row_tiles, int* split_blocks, int* splits) {
+// How the shared prefix is cut for the packed product, and how many CTAs it gets: the others of the machine's
+// SMs are left to the streaming kernel, which starts beside it (own keys from HBM under the product's arithmetic).
+// Both times are estimated, in us, from what the kernels measure on an idle machine: 2.0 per block of 128 keys and
+// 256 rows (1.6 with one live half), 3 per tile and 6 per launch here; 0.3 per 16 KB that one SM streams, 5 per launch.
+struct PackedPlan {
+  int seqs_per_half, row_tiles, split_blocks, splits, ctas;
+};
+
+PackedPlan plan_packed(const CacheAttn& a) {
+  PackedPlan p;
   const int per_seq = a.G * a.Sq;
   const int fit = HALF / per_seq;
-  *seqs_per_half = fit < a.B ? fit : a.B;
-  *row_tiles = (a.B + 2 * *seqs_per_half - 1) / (2 * *seqs_per_half);
+  p.seqs_per_half = fit < a.B ? fit : a.B;
+  p.row_tiles = (a.B + 2 * p.seqs_per_half - 1) / (2 * p.seqs_per_half);
   const int blocks = (a.P + BKV - 1) / BKV;
-  const int64_t tasks = static_cast<int64_t>(a.Hkv) * *row_tiles;
-  int64_t n = sm_count() / tasks;
-  n = n < 1 ? 1 : n > blocks ? blocks : n;
-  *split_blocks = static_cast<int>((blocks + n - 1) / n);
-  *splits = (blocks + *split_blocks - 1) / *split_blocks;
+  const int64_t tasks = static_cast<int64_t>(a.Hkv) * p.row_tiles;
+  const int sms = sm_count();
+  const float per_block = p.seqs_per_half < a.B ? 2.0f : 1.6f;
+  const float stream_us = 0.3f * stream_units(a) * a.D / 128;
+  float best = INFINITY;
+  for (int eighth = 4; eighth <= 8; ++eighth) {
+    const int ctas = eighth == 8 ? sms - sms / 16 : sms * eighth / 8;
+    for (int rounds = 1; rounds <= 3; ++rounds) {
+      int64_t splits = rounds * ctas / tasks;
+      splits = splits < 1 ? 1 : splits > blocks ? blocks : splits;
+      const int split_blocks = static_cast<int>((blocks + splits - 1) / splits);
+      splits = (blocks + split_blocks - 1) / split_blocks;
+      const float tile_us = 6.0f + (tasks * splits + ctas - 1) / ctas * (split_blocks * per_block + 3.0f);
+      const float us = fmaxf(tile_us, 5.0f + stream_us / (sms - ctas));
+      if (us < best) {
+        best = us;
+        p.split_blocks = split_blocks;
+        p.splits = static_cast<int>(splits);
+        p.ctas = static_cast<int>(tasks * splits < ctas ? tasks * splits : ctas);
+      }
+    }
+  }
+  if (getenv("TA_CTAS")) {
+    p.ctas = atoi(getenv("TA_CTAS"));
+    int64_t splits = atoi(getenv("TA_ROUNDS")) * p.ctas / tasks;
+    splits = splits < 1 ? 1 : splits > blocks ? blocks : splits;
+    p.split_blocks = static_cast<int>((blocks + splits - 1) / splits);
+    p.splits = (blocks + p.split_blocks - 1) / p.split_blocks;
+    if (p.ctas > tasks * p.splits) p.ctas = tasks * p.splits;
+  }
+  return p;
 }
 
+int packed_ctas(const CacheAttn& a) { return plan_packed(a).ctas; }
+
 size_t packed_workspace(const CacheAttn& a) {
-  int seqs, tiles, blocks, splits;
-  plan_packed(a, &seqs, &tiles, &blocks, &splits);
-  const size_t rows = static_cast<size_t>(a.B) * a.Sq * a.G;
-  return kTileCounterBytes + static_cast<size_t>(splits) * a.Hkv * rows * (a.D + 1) * sizeof(float);
+  const PackedPlan p = plan_packed(a);
+  return kTileCounterBytes + static_cast<size_t>(p.splits) * a.Hkv * p.row_tiles * 2 * HALF * (a.D + 1) * sizeof(float);
 }
 
 int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream) {
   TileArgs t = {};
   t.a = a;
-  plan_packed(a, &t.seqs_per_half, &t.n_qtiles, &t.split_blocks, &t.splits);
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.G;
+  const PackedPlan plan = plan_packed(a);
+  t.seqs_per_half = plan.seqs_per_half;
+  t.n_qtiles = plan.row_tiles;
+  t.split_blocks = plan.split_blocks;
+  t.splits = plan.splits;
+  const int64_t rows = static_cast<int64_t>(plan.row_tiles) * 2 * HALF;
+  if (rows > 0x3fffffff) { set_error("attention: too many sequences"); return CDR_ERR_UNSUPPORTED; }
   t.part_rows = static_cast<int>(rows);
   t.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kTileCounterBytes);
   t.part_lse = t.part_o + static_cast<size_t>(t.splits) * a.Hkv * rows * a.D;
   if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, a.Sq, a.G, t.seqs_per_half, true)) return rc;
   if (int rc = map_prefix(t)) return rc;
-  *part = PrefixPartials{t.part_o, t.part_lse, t.splits, t.part_rows};
-  return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, ws, stream);
+  *part = PrefixPartials{t.part_o, t.part_lse, t.splits, t.part_rows, t.seqs_per_half};
+  return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, plan.ctas, ws, stream);
 }
 
 }  // namespace cdr
