@@ -55,6 +55,7 @@ struct StreamArgs {
   int* status;
   PrefixPartials part;     // splits > 0: the prefix is already done
   float *slot_o, *slot_ml; // parts: [slot][row of the task][D] and [..][2] = (maximum, sum)
+  int* cum;                // [groups + 1] cumulated units, left for the second kernel (lengths given)
   int n_warps;             // shares
   int cluster;             // CTAs per task (CLUSTER)
   int m_tiles;             // tasks per (sequence, key head)
@@ -234,13 +235,34 @@ struct RowSum {
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, top = -INFINITY;
 
   __device__ __forceinline__ void join(float m, float l, float4 u, float4 v) {
-    if (m == -INFINITY) return;
+    const bool none = m == -INFINITY;              // a part that saw nothing may hold anything
     const float m_new = fmaxf(top, m);
-    const float f0 = top == -INFINITY ? 0.0f : ex2(top - m_new), f1 = ex2(m - m_new);
+    const float f0 = top == -INFINITY ? 0.0f : ex2(top - m_new), f1 = none ? 0.0f : ex2(m - m_new);
+    if (none) { l = 0.0f; u = v = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
     top = m_new;
     sum = f0 * sum + f1 * l;
     acc[0] = f0 * acc[0] + f1 * u.x; acc[1] = f0 * acc[1] + f1 * u.y; acc[2] = f0 * acc[2] + f1 * u.z; acc[3] = f0 * acc[3] + f1 * u.w;
     acc[4] = f0 * acc[4] + f1 * v.x; acc[5] = f0 * acc[5] + f1 * v.y; acc[6] = f0 * acc[6] + f1 * v.z; acc[7] = f0 * acc[7] + f1 * v.w;
+  }
+  // parts first, first + step, ... < n; get(i, &o) returns (maximum, sum) of part i and where its 8 columns are.  Four
+  // parts are fetched before the first of them is used.
+  template <typename Get>
+  __device__ __forceinline__ void join_parts(int first, int step, int n, Get get) {
+    for (int i0 = first; i0 < n; i0 += 4 * step) {
+      float2 ml[4];
+      float4 u[4], v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * step;
+        const float* o;
+        ml[k] = get(i < n ? i : i0, &o);
+        u[k] = reinterpret_cast<const float4*>(o)[0];
+        v[k] = reinterpret_cast<const float4*>(o)[1];
+        if (i >= n) ml[k].x = -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) join(ml[k].x, ml[k].y, u[k], v[k]);
+    }
   }
   // with the lane whose number differs in bit x (every lane of the warp calls this)
   __device__ __forceinline__ void join_lane(int x) {
@@ -260,6 +282,18 @@ struct RowSum {
     for (int e = 0; e < 4; ++e) w[e] = pack16<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
     const int64_t e0 = b * a.so.b + hq * a.so.h + static_cast<int64_t>(i) * a.so.s + d;
     *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + e0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// part n of the shared prefix for one row and 8 of its columns
+struct PrefixGet {
+  const PrefixPartials& part;
+  int64_t row;             // of split 0
+  int kv_heads, dim, column;
+  __device__ __forceinline__ float2 operator()(int n, const float** o) const {
+    const int64_t e = static_cast<int64_t>(n) * kv_heads * part.rows + row;
+    *o = part.o + e * dim + column;
+    return make_float2(part.lse[e], 1.0f);
   }
 };
 
@@ -328,6 +362,8 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
     share = warp * cs + rank;
   } else {
     total = cumulate_units<L::THREADS>(args, cum, warp_sum, &uniform);
+    if (a.lengths && blockIdx.x == 0)
+      for (int e = threadIdx.x; e <= args.groups; e += L::THREADS) args.cum[e] = e < args.groups ? cum[e] : total;
     share = warp * gridDim.x + blockIdx.x;               // neighbouring shares on different SMs
   }
   const Shares shares(total, n_warps);
@@ -587,27 +623,17 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
       const int r = r_first + row, i = r / a.G, gi = r - i * a.G;
       RowSum sum;
       if (live && lt.len - a.Sq + i >= 0) {
-#pragma unroll 3
-        for (int n = sub; n < n_parts; n += tpp) {
+        sum.join_parts(sub, tpp, n_parts, [&](int n, const float** o) {
           const int wn = n % L::WARPS, cn = n / L::WARPS;
           const float2* pml = &sm_ml[wn][row];
-          const float* po = reinterpret_cast<const float*>(smem + wn * (SA_STAGES * L::STAGE_BYTES)) + row * PITCH + d;
+          *o = reinterpret_cast<const float*>(smem + wn * (SA_STAGES * L::STAGE_BYTES)) + row * PITCH + d;
           if (cs > 1) {
             pml = static_cast<const float2*>(__cluster_map_shared_rank(pml, cn));
-            po = static_cast<const float*>(__cluster_map_shared_rank(po, cn));
+            *o = static_cast<const float*>(__cluster_map_shared_rank(*o, cn));
           }
-          const float2 ml = *pml;
-          const float4 u = reinterpret_cast<const float4*>(po)[0], v = reinterpret_cast<const float4*>(po)[1];
-          sum.join(ml.x, ml.y, u, v);
-        }
-        const int prow = args.part.splits ? args.part.row_of(a, lt.b, i, gi) : 0;
-#pragma unroll 4
-        for (int n = sub; n < args.part.splits; n += tpp) {
-          const size_t e = (static_cast<size_t>(n) * a.Hkv + lt.hkv) * args.part.rows + prow;
-          const float4* src = reinterpret_cast<const float4*>(args.part.o + e * HD + d);
-          const float4 u = src[0], v = src[1];
-          sum.join(args.part.lse[e], 1.0f, u, v);
-        }
+          return *pml;
+        });
+        if (behind_prefix) sum.join_parts(sub, tpp, args.part.splits, PrefixGet{args.part, args.part.row_of(a, lt.b, i, gi) + static_cast<int64_t>(lt.hkv) * args.part.rows, a.Hkv, HD, d});
       }
       for (int x = 1; x < tpp; x *= 2) sum.join_lane(x);
       if (live && sub == 0) sum.template store<BF16>(a, lt.b, lt.hkv * a.G + gi, i, d);
@@ -624,12 +650,7 @@ template <int HD, bool BF16>
 __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_constant__ StreamArgs args, int tpr) {
   constexpr int VECS = HD / 8;
   __shared__ float sm_acc[CA_THREADS / 32][VECS][8], sm_ms[CA_THREADS / 32][VECS][2];
-  extern __shared__ int cum[];
-  __shared__ int warp_sum[CA_THREADS / 32];
   const CacheAttn& a = args.a;
-  // the list of units needs only the lengths, which were there before the first of the kernels started
-  int uniform;
-  const int total = cumulate_units<CA_THREADS>(args, cum, warp_sum, &uniform);
   const int prefix = args.part.splits == 0 ? a.P : 0;
   const int rows = a.G * a.Sq;
   const int64_t row_all = static_cast<int64_t>(blockIdx.x) * (CA_THREADS / tpr) + threadIdx.x / tpr;
@@ -645,12 +666,17 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
   // the task's units, and the shares that hold them
   const int len = sequence_length(a, b);
   const int per_head = head_units(a, prefix, len, args.m_tiles);
-  int first;
-  if (uniform) {
+  // (the lengths were there before the first of the kernels started; what that one left is there after the wait)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  int first, total;
+  if (!a.lengths) {
     first = per_head * (b * a.Hkv + hkv);
+    total = per_head * a.Hkv * a.B;
   } else {
     const int e = b / args.group;
-    first = (a.lengths ? cum[e] : 0) + per_head * hkv;
+    first = args.cum[e] + per_head * hkv;
+    total = args.cum[args.groups];
     for (int x = e * args.group; x < b; ++x) first += head_units(a, prefix, sequence_length(a, x), args.m_tiles) * a.Hkv;
   }
   for (int x = 0; x < mt; ++x) first += key_ranges(a, prefix, len, x).n_total;
@@ -668,26 +694,14 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
   const int task = (b * a.Hkv + hkv) * args.m_tiles + mt;
 
   RowSum sum;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;");
   if (sees) {
-#pragma unroll 4
-    for (int w = w0 + sub; w <= w1; w += nsub) {
+    sum.join_parts(w0 + sub, nsub, w1 + 1, [&](int w, const float** o) {
       const int64_t slot = w0 == w1 ? 2LL * args.n_warps + task : 2LL * w + (w == w0 ? first_slot : 0);
       const int64_t at = slot * args.rows_cap + row;
-      const float4* src = reinterpret_cast<const float4*>(args.slot_o + at * HD + vec * 8);
-      const float2 ml = *reinterpret_cast<const float2*>(args.slot_ml + at * 2);
-      const float4 u = src[0], v = src[1];
-      sum.join(ml.x, ml.y, u, v);
-    }
-    const int prow = behind_prefix ? args.part.row_of(a, b, i, gi) : 0;
-#pragma unroll 4
-    for (int n = sub; n < args.part.splits; n += nsub) {
-      const size_t e = (static_cast<size_t>(n) * a.Hkv + hkv) * args.part.rows + prow;
-      const float4* src = reinterpret_cast<const float4*>(args.part.o + e * HD + vec * 8);
-      const float4 u = src[0], v = src[1];
-      sum.join(args.part.lse[e], 1.0f, u, v);
-    }
+      *o = args.slot_o + at * HD + vec * 8;
+      return *reinterpret_cast<const float2*>(args.slot_ml + at * 2);
+    });
+    if (behind_prefix) sum.join_parts(sub, nsub, args.part.splits, PrefixGet{args.part, args.part.row_of(a, b, i, gi) + static_cast<int64_t>(hkv) * args.part.rows, a.Hkv, HD, vec * 8});
   }
   // lanes of a warp with the same columns, then the row's warps
   for (int x = VECS; x < 32; x *= 2) sum.join_lane(x);
@@ -744,8 +758,10 @@ StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
   return p;
 }
 
+size_t table_bytes(const StreamPlan& p) { return (static_cast<size_t>(p.groups + 1) * sizeof(int) + 255) / 256 * 256; }
+
 size_t stream_bytes(const CacheAttn& a, const StreamPlan& p) {
-  return static_cast<size_t>(p.slots) * p.rows_cap * (a.D + 2) * sizeof(float);
+  return p.cluster ? 0 : table_bytes(p) + static_cast<size_t>(p.slots) * p.rows_cap * (a.D + 2) * sizeof(float);
 }
 
 template <int HD, bool BF16>
@@ -785,7 +801,7 @@ int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStr
   const int64_t rows = static_cast<int64_t>(s.a.B) * s.a.Hq * s.a.Sq;
   cfg.gridDim = dim3(static_cast<unsigned>((rows + CA_THREADS / tpr - 1) / (CA_THREADS / tpr)), 1, 1);
   cfg.blockDim = dim3(CA_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = table;
+  cfg.dynamicSmemBytes = 0;
   CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, combine_parts_kernel<HD, BF16>, s, tpr));
   return CDR_OK;
 }
@@ -812,7 +828,8 @@ int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void
     if (int rc = make_map(&s.tmap_pk, a.pk, a, a.P, a.Hkv, 1, a.spk)) return rc;
     if (int rc = make_map(&s.tmap_pv, a.pv, a, a.P, a.Hkv, 1, a.spv)) return rc;
   }
-  s.slot_o = static_cast<float*>(ws);
+  s.cum = static_cast<int*>(ws);
+  s.slot_o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + table_bytes(p));
   s.slot_ml = s.slot_o + p.slots * p.rows_cap * a.D;
   s.n_warps = p.n_warps;
   s.cluster = p.cluster;
@@ -820,10 +837,11 @@ int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void
   s.group = p.group;
   s.groups = p.groups;
   s.rows_cap = p.rows_cap;
-  // threads per row of the second kernel: by the parts a row may have
+  // threads per row of the second kernel: by the parts a row may have (a CTA per row pays only where there are few rows:
+  // 2048 rows of 24 parts take 26 us so, 12 with two warps per row)
   const int64_t per_task = p.tasks ? p.units / p.tasks : 0, per_warp = p.units / p.n_warps + 1;
   const int64_t parts = per_task / per_warp + 1 + part.splits;
-  const int tpr = parts <= 4 ? 32 : parts <= 16 ? 64 : 256;
+  const int tpr = rows <= 2 * sm_count() && parts > 16 ? 256 : parts <= 8 ? 32 : 64;
   if (a.D == 128) return a.bf16 ? launch_stream_cfg<128, true>(s, p, tpr, stream) : launch_stream_cfg<128, false>(s, p, tpr, stream);
   return a.bf16 ? launch_stream_cfg<64, true>(s, p, tpr, stream) : launch_stream_cfg<64, false>(s, p, tpr, stream);
 }

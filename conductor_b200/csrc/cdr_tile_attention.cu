@@ -19,7 +19,6 @@
 //     scratch in fp32, where the streaming kernel joins them with the sequences' own keys.
 #include <cuda.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include "cdr_attention_softmax.cuh"
 #include "cdr_cache_attention.cuh"
@@ -700,8 +699,9 @@ int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
 
 // How the shared prefix is cut for the packed product, and how many CTAs it gets: the others of the machine's
 // SMs are left to the streaming kernel, which starts beside it (own keys from HBM under the product's arithmetic).
-// Both times are estimated, in us, from what the kernels measure on an idle machine: 2.0 per block of 128 keys and
-// 256 rows (1.6 with one live half), 3 per tile and 6 per launch here; 0.3 per 16 KB that one SM streams, 5 per launch.
+// Both times are estimated, in us, from what the kernels measure on this machine: here 1.95 per block of 128 keys and 256
+// rows (1.6 with one live half), 3 per tile and 5 per launch; there 0.19 per 16 KB and SM, 8 per launch.  64 sequences of 32
+// heads behind 16384 keys, 512 own ones: 71 us one after the other, 46.6 with 88 CTAs here, 52.9 with 112, 72 with 120.
 struct PackedPlan {
   int seqs_per_half, row_tiles, split_blocks, splits, ctas;
 };
@@ -715,18 +715,18 @@ PackedPlan plan_packed(const CacheAttn& a) {
   const int blocks = (a.P + BKV - 1) / BKV;
   const int64_t tasks = static_cast<int64_t>(a.Hkv) * p.row_tiles;
   const int sms = sm_count();
-  const float per_block = p.seqs_per_half < a.B ? 2.0f : 1.6f;
-  const float stream_us = 0.3f * stream_units(a) * a.D / 128;
+  const float per_block = p.seqs_per_half < a.B ? 1.95f : 1.6f;
+  const float stream_us = 0.19f * stream_units(a) * a.D / 128;
   float best = INFINITY;
   for (int eighth = 4; eighth <= 8; ++eighth) {
-    const int ctas = eighth == 8 ? sms - sms / 16 : sms * eighth / 8;
-    for (int rounds = 1; rounds <= 3; ++rounds) {
+    const int ctas = ((eighth == 8 ? sms - sms / 16 : sms * eighth / 8) + 3) / 4 * 4;
+    for (int rounds = 1; rounds <= 2; ++rounds) {
       int64_t splits = rounds * ctas / tasks;
       splits = splits < 1 ? 1 : splits > blocks ? blocks : splits;
       const int split_blocks = static_cast<int>((blocks + splits - 1) / splits);
       splits = (blocks + split_blocks - 1) / split_blocks;
-      const float tile_us = 6.0f + (tasks * splits + ctas - 1) / ctas * (split_blocks * per_block + 3.0f);
-      const float us = fmaxf(tile_us, 5.0f + stream_us / (sms - ctas));
+      const float tile_us = 5.0f + (tasks * splits + ctas - 1) / ctas * (split_blocks * per_block + 3.0f);
+      const float us = fmaxf(tile_us, 8.0f + stream_us / (sms > ctas ? sms - ctas : 1));
       if (us < best) {
         best = us;
         p.split_blocks = split_blocks;
@@ -734,14 +734,6 @@ PackedPlan plan_packed(const CacheAttn& a) {
         p.ctas = static_cast<int>(tasks * splits < ctas ? tasks * splits : ctas);
       }
     }
-  }
-  if (getenv("TA_CTAS")) {
-    p.ctas = atoi(getenv("TA_CTAS"));
-    int64_t splits = atoi(getenv("TA_ROUNDS")) * p.ctas / tasks;
-    splits = splits < 1 ? 1 : splits > blocks ? blocks : splits;
-    p.split_blocks = static_cast<int>((blocks + splits - 1) / splits);
-    p.splits = (blocks + p.split_blocks - 1) / p.split_blocks;
-    if (p.ctas > tasks * p.splits) p.ctas = tasks * p.splits;
   }
   return p;
 }
