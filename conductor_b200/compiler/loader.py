@@ -79,6 +79,16 @@ def load_library(build_if_missing: bool = False) -> ctypes.CDLL:
     return lib
 
 
+def load_call_module():
+    """The compiled host side of direct operator calls (``csrc/cdr_torch.cpp``)."""
+    try:
+        from ..csrc import _cdr_torch
+    except ImportError as exc:
+        raise DeviceError("the call module of conductor_b200.ops is missing or does not fit this torch "
+                          f"({exc}); run `python -m conductor_b200.csrc.build`") from exc
+    return _cdr_torch
+
+
 def unload_library() -> None:
     global _lib
     _lib = None

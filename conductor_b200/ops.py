@@ -31,7 +31,7 @@ import torch
 
 from .codegen.kernel_templates import CdrLaunchItem, CdrTensor, prefix_attention_launch, window_attention_launch
 from .compiler.executor import attention_view_ok, get_executor, make_descriptors, raise_for_status
-from .compiler.loader import load_library
+from .compiler.loader import load_call_module, load_library
 from .utils.exceptions import DeviceError, ExecutionError
 from .utils.type_mapping import to_cdr_dtype
 
@@ -62,20 +62,21 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
 # ---------------------------------------------------------------- direct calls
 # A decode step takes about as long on the GPU as a few Python statements do on the host, so a repeated
 # call (same shapes, strides, types and parameters) only refreshes pointers: its descriptors, parameter
-# block and launch item are kept per thread.  Nothing of the tensors themselves is kept.
+# block and launch item are kept per thread, and the compiled call module checks the tensors against them, takes
+# output and scratch from torch's caching allocator and launches.  Nothing of the tensors themselves is kept.
 _calls = threading.local()
 _MAX_CALLS = 256
 
 
 class _Call:
-    """A marshalled launch: one ``cdr_launch_item`` whose pointers are set before every use."""
+    """A marshalled launch for tensors of given shapes, strides and types on one device."""
 
-    __slots__ = ("name", "item", "address", "inputs", "output", "workspace_bytes", "bytes", "shape", "dtype", "like", "launch_many", "keep")
+    __slots__ = ("name", "call", "keep")
 
     def __init__(self, launch, tensors):
         lib = load_library()
-        out = torch.empty(launch.out_shapes[0], dtype=launch.out_dtypes[0], device="meta")
         in_desc, out_desc = make_descriptors(tensors), (CdrTensor * 1)()
+        out = torch.empty(launch.out_shapes[0], dtype=launch.out_dtypes[0], device="meta")
         out_desc[0].dtype, out_desc[0].rank = to_cdr_dtype(out.dtype), out.dim()
         for i, (n, st) in enumerate(zip(out.shape, out.stride())):
             out_desc[0].shape[i], out_desc[0].stride[i] = n, st
@@ -85,80 +86,60 @@ class _Call:
         with torch.cuda.device(tensors[0].device):
             rc = lib.cdr_workspace_bytes(launch.template, in_desc, len(tensors), out_desc, 1, params, size, ctypes.byref(need))
         raise_for_status(lib, rc, launch.name)
-        self.name, self.workspace_bytes = launch.name, need.value
-        self.shape, self.dtype, self.like = tuple(out.shape), out.dtype, tensors[0].is_contiguous()
-        self.bytes = torch.empty(0, dtype=torch.uint8, device=tensors[0].device)
-        self.launch_many = lib.cdr_launch_many
-        self.inputs, self.output = list(in_desc), out_desc[0]
-        self.item = CdrLaunchItem(launch.template, len(tensors), 1, 0, ctypes.addressof(in_desc), ctypes.addressof(out_desc),
-                                  params.value, size, None, need.value)
-        self.address = ctypes.addressof(self.item)
-        self.keep = (launch, in_desc, out_desc)
+        item = CdrLaunchItem(launch.template, len(tensors), 1, 0, ctypes.addressof(in_desc), ctypes.addressof(out_desc),
+                             params.value, size, None, need.value)
+        self.name = launch.name
+        self.call = load_call_module().Call(ctypes.addressof(item), ctypes.addressof(in_desc), ctypes.addressof(out_desc),
+                                    ctypes.cast(lib.cdr_launch_many, ctypes.c_void_p).value, tuple(tensors))
+        self.keep = (launch, item, in_desc, out_desc)
 
-    def __call__(self, q, pointers, index):
-        # the output is contiguous; empty_like is the cheaper way to it where q is
-        out = torch.empty_like(q) if self.like else torch.empty(self.shape, dtype=self.dtype, device=q.device)
-        for desc, p in zip(self.inputs, pointers):
-            desc.data = p
-        self.output.data = out.data_ptr()
-        if self.workspace_bytes:
-            # of this call alone: it goes back to the current stream's pool once the launch is enqueued
-            ws = self.bytes.new_empty(self.workspace_bytes)
-            self.item.workspace = ws.data_ptr()
-        if _current_device() == index:
-            rc = self.launch_many(self.address, 1, _raw_stream(index), None)
-        else:
-            with torch.cuda.device(index):
-                rc = self.launch_many(self.address, 1, _raw_stream(index), None)
-        if rc:
-            raise_for_status(load_library(), rc, self.name)
+    def __call__(self, tensors):
+        """The output, or None when the tensors are not the ones this call was made for."""
+        out = self.call.run(*tensors)
+        if out.__class__ is int:
+            raise_for_status(load_library(), out, self.name)
         return out
 
 
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 def _run(name, build, params, tensors):
-    """Run one of the operators on `tensors`: everything the library's checks depend on is in the key, so a
-    kept call has passed them; only what may change between two such calls is looked at here."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
-                                     "torch.no_grad() or detach the inputs", kernel_name=name)
-    key = (name, params, *[(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
     try:
-        call = _calls.cache.get(key)
-    except AttributeError:
-        _calls.cache, call = {}, None
+        call = _calls.last.get((name, params))
+    except AttributeError:                         # this thread's first call
+        _calls.last, _calls.cache, call = {}, {}, None
     if call is not None:
-        pointers = [t.data_ptr() for t in tensors]
-        low = 0
-        for p in pointers:
-            low |= p
-        if not low & 15:
-            q = tensors[0]
-            return call(q, pointers, q.get_device())
-    return _first_run(name, build, params, tensors, key)
+        out = call(tensors)
+        if out is not None:
+            return out
+    return _other_run(name, build, params, tensors)
 
 
-def _first_run(name, build, params, tensors, key):
+def _other_run(name, build, params, tensors):
+    """A call that is not the last one of its parameters again: found among the kept ones, or made."""
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")
     for t in tensors:
         if t.device != device:
             raise ExecutionError(f"{name}: tensors on {device} and {t.device}", kernel_name=name)
-    launch = build(tensors[0], *params)
-    if any(t.data_ptr() % 16 or not attention_view_ok(t) for t in tensors):
-        return get_executor().execute(launch, tensors)[0]      # gathers what cannot be read in place
-    call = _Call(launch, tensors)
-    if len(_calls.cache) >= _MAX_CALLS:
-        _calls.cache.clear()
-    _calls.cache[key] = call
-    return call(tensors[0], [t.data_ptr() for t in tensors], device.index)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
+                                 "torch.no_grad() or detach the inputs", kernel_name=name)
+    key = (name, params, *[(t.shape, t.stride(), t.dtype) for t in tensors], device)
+    call = _calls.cache.get(key)
+    out = call(tensors) if call is not None else None
+    if out is None:
+        launch = build(tensors[0], *params)
+        if any(not attention_view_ok(t) for t in tensors):
+            return get_executor().execute(launch, tensors)[0]      # gathers what cannot be read in place
+        if len(_calls.cache) >= _MAX_CALLS:
+            _calls.cache.clear()
+            _calls.last.clear()
+        call = _calls.cache[key] = _Call(launch, tensors)
+        out = call(tensors)
+        if out is None:                                            # a tensor subclass: the general way
+            return get_executor().execute(launch, tensors)[0]
+    _calls.last[(name, params)] = call
+    return out
 
 
 def _build_window(q, window, sinks, has_lengths, scale):

@@ -129,6 +129,26 @@ def test_arguments_are_checked_by_the_library(built_library):
         assert prefix(a, b)[0] == -1
 
 
+def test_call_module_takes_only_the_tensors_it_was_made_for(built_library):
+    """The compiled side of direct calls: anything else than the tensors of the first call is left to the caller."""
+    from conductor.compiler.loader import load_call_module
+    from conductor_b200.csrc.build import build_call_module
+
+    build_call_module()
+    module = load_call_module()
+    item, ins, out = kt.CdrLaunchItem(), (kt.CdrTensor * 3)(), (kt.CdrTensor * 1)()
+    q, k, v = cache()
+    call = module.Call(ctypes.addressof(item), ctypes.addressof(ins), ctypes.addressof(out), 0, (q, k, v))
+    shifted = torch.zeros(q.numel() + 1, dtype=q.dtype)[1:].view(q.shape)
+    for bad in ((q, k), (q, k, v, v), (q, k, v[:1]), (q.half(), k, v), (q, k, v.transpose(1, 2).contiguous().transpose(1, 2)),
+                (shifted, k, v), (q.clone().requires_grad_(), k, v), (q, k, None)):
+        assert call.run(*bad) is None
+    with pytest.raises(TypeError):
+        module.Call(1, 2, 3, 4, (1, 2))
+    with pytest.raises(TypeError):
+        module.Call(1, 2)
+
+
 def test_views_the_kernels_read_in_place():
     base = torch.zeros(2, 9, 4, 64, dtype=torch.bfloat16)
     assert attention_view_ok(base) and attention_view_ok(base.transpose(1, 2)) and attention_view_ok(base[:, 3:7, 1:2])
