@@ -78,19 +78,13 @@ struct Tile {
   int p0, np;                // prefix blocks
   int ns, wstart;            // own blocks: [0, ns) and [wstart, ...)
   int n_iter;
-  int live[2], fw[2], lw[2]; // the half has rows that see keys; first and last own block of their windows
+  int live[2];               // the half has rows that see keys
+  int pre[2], wa[2], wb[2];  // it takes part in entries [0, pre) and [wa, wb]
   int light[2];              // entry 0 holds nothing but at most 32 sinks for the half
 
   __device__ __forceinline__ int own_block(int j) const { const int o = j - np; return o < ns ? o : wstart + o - ns; }
-  // a half with these values has rows that see keys of entry j
-  __device__ __forceinline__ bool active(int half_live, int half_fw, int half_lw, int j) const {
-    if (!half_live) return false;
-    if (j < np) return true;
-    const int kb = own_block(j);
-    return kb <= half_lw && (kb < ns || kb >= half_fw);
-  }
   __device__ __forceinline__ bool active(int h, int j) const {   // h: known to the compiler
-    return active(live[h], fw[h], lw[h], j);
+    return j < pre[h] || (j >= wa[h] && j <= wb[h]);
   }
 };
 
@@ -138,6 +132,10 @@ __device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len,
     r.n_iter = r.np;
     r.live[0] = 1;
     r.live[1] = r.b + t.seqs_per_half < a.B;
+    r.pre[0] = r.np;
+    r.pre[1] = r.live[1] ? r.np : 0;
+    r.wa[0] = r.wa[1] = 0;
+    r.wb[0] = r.wb[1] = -1;
     return;
   }
   // heads in groups that fill the machine; inside a group the tiles from the last to the first, heads
@@ -152,25 +150,35 @@ __device__ __forceinline__ void decode_tile(const TileArgs& t, int idx, int len,
   r.hq = bh % a.Hq;
   r.hkv = r.hq / a.G;
   r.off = len - a.Sq;
+  int fw[2], lw[2];          // first and last own block that the rows' windows touch
   int wlo = 0x7fffffff, whi = -1, p_max = -1;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int row0 = r.q0 + h * HALF;
     const int last = r.off + min(row0 + HALF, a.Sq) - 1;
     r.live[h] = row0 < a.Sq && last >= 0;
-    r.fw[h] = max(max(r.off + row0, 0) - a.window + 1, 0) / BKV;
-    r.lw[h] = last / BKV;
-    if (r.live[h]) { wlo = min(wlo, r.fw[h]); whi = max(whi, r.lw[h]); p_max = max(p_max, last); }
+    fw[h] = max(max(r.off + row0, 0) - a.window + 1, 0) / BKV;
+    lw[h] = last / BKV;
+    if (r.live[h]) { wlo = min(wlo, fw[h]); whi = max(whi, lw[h]); p_max = max(p_max, last); }
+    r.pre[h] = r.wa[h] = 0;
+    r.wb[h] = -1;
   }
   r.p0 = r.np = r.ns = r.wstart = r.n_iter = r.light[0] = r.light[1] = 0;
   if (p_max >= 0) {
     r.np = (a.P + BKV - 1) / BKV;
     const bool few = r.np == 0 && a.sinks > 0 && a.sinks <= SINK_COLS;
-    r.light[0] = few && r.live[0] && r.fw[0] > 0;
-    r.light[1] = few && r.live[1] && r.fw[1] > 0;
+    r.light[0] = few && r.live[0] && fw[0] > 0;
+    r.light[1] = few && r.live[1] && fw[1] > 0;
     r.ns = (min(a.sinks, p_max + 1) + BKV - 1) / BKV;
     r.wstart = max(r.ns, wlo);
     r.n_iter = r.np + r.ns + max(whi - r.wstart + 1, 0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!r.live[h]) continue;
+      r.pre[h] = r.np + min(r.ns, lw[h] + 1);
+      r.wa[h] = r.np + r.ns + max(fw[h] - r.wstart, 0);
+      r.wb[h] = r.np + r.ns + lw[h] - r.wstart;
+    }
   }
 }
 
@@ -334,10 +342,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         bool k_ready = false;
         unsigned char* v_tile = smem + L::KV_OFF + ((ring + vt) % KV_STAGES) * L::TILE_BYTES;
         const uint32_t v_addr = sm100::smem_u32(v_tile);
-        if (!PACKED && j >= r.np) {
+        if (!PACKED && !next && j >= r.np && len < a.Skv) {
+          // the list ends with the block of the last position that some row of the tile sees.
           // V rows behind the sequence's end: a weight of 0 must not meet what the cache holds there
           const int keep = len - r.own_block(j) * BKV;
-          if (keep < BKV && len < a.Skv) {
+          if (keep < BKV) {
             for (int x = lane; x < (BKV - keep) * (HD / 8); x += 32) {
               const int row = keep + x / (HD / 8), piece = x % (HD / 8);
               *reinterpret_cast<uint4*>(v_tile + (piece >> 3) * (128 * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -419,13 +428,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const int p_first = r.off + row0, p_last = r.off + min(row0 + HALF, a.Sq) - 1;
       const int pos = p_first + row_in_half;         // this row's position (PACKED: unused)
       // (selected, not indexed: an index that the compiler does not know would put the tile into local memory)
-      const int live = g ? r.live[1] : r.live[0], fw = g ? r.fw[1] : r.fw[0], lw = g ? r.lw[1] : r.lw[0],
-                light = g ? r.light[1] : r.light[0];
+      const int live = g ? r.live[1] : r.live[0], light = g ? r.light[1] : r.light[0];
+      const int pre = g ? r.pre[1] : r.pre[0], wa = g ? r.wa[1] : r.wa[0], wb = g ? r.wb[1] : r.wb[0];
       float m_ref = -INFINITY, l0 = 0.0f, l1 = 0.0f;
       bool first = true;
 
       for (int j = 0; j < r.n_iter; ++j) {
-        if (!r.active(live, fw, lw, j)) continue;
+        if (j >= pre && (j < wa || j > wb)) continue;
         if (!sm100::mbar_wait(&bars[B_SFULL + g], n & 1)) { sm100::report_timeout(t.status, 52); ok = false; break; }
         ++n;
         sm100::tc_fence_after();

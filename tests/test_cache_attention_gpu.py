@@ -1,9 +1,12 @@
 """window_attention and prefix_attention on a GPU against their definition in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 
 import conductor
 from cache_attention_ref import check, reference
+from conductor.compiler.loader import load_library
 from conductor.utils.exceptions import DeviceError, ExecutionError, UnsupportedOperationError
 
 pytestmark = pytest.mark.gpu
@@ -22,6 +25,14 @@ def cache(B, Hq, Hkv, Sq, Skv, D, dtype=torch.bfloat16, seed=0):
 
 def lens(*n, dtype=torch.int32):
     return torch.tensor(n, dtype=dtype, device=DEV)
+
+
+@pytest.fixture(autouse=True, scope="module")
+def no_wait_gave_up():
+    """Every device-side wait of these tests ended by its signal, not by its limit."""
+    yield
+    word = ctypes.c_int(0)
+    assert load_library().cdr_device_status(ctypes.byref(word), 1) == 0, hex(word.value)
 
 
 SHAPES = [
@@ -66,7 +77,8 @@ def test_lengths(Hq, Hkv, Sq, Skv, index):
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,Sq,P,D", [(2, 8, 8, 1, 900, 64), (20, 32, 8, 1, 600, 128), (130, 8, 1, 1, 1000, 64), (9, 14, 2, 3, 513, 128),
-                                             (70, 4, 4, 5, 300, 64), (300, 2, 2, 1, 128, 128), (3, 16, 1, 8, 257, 64), (2, 16, 1, 9, 257, 64), (5, 200, 1, 1, 140, 128)])
+                                             (70, 4, 4, 5, 300, 64), (300, 2, 2, 1, 128, 128), (3, 16, 1, 8, 257, 64), (2, 16, 1, 9, 257, 64), (5, 200, 1, 1, 140, 128),
+                                             (13, 14, 2, 3, 5003, 64), (33, 32, 4, 1, 3000, 128), (257, 8, 2, 1, 2000, 64)])
 def test_prefix_of_many_sequences(B, Hq, Hkv, Sq, P, D):
     q, k, v = cache(B, Hq, Hkv, Sq, 40, D, seed=B)
     lengths = torch.arange(B, device=DEV) * 7 % 41
