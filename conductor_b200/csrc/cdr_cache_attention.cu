@@ -33,7 +33,7 @@
 namespace cdr {
 
 int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const int64_t* dims, const int64_t* strides,
-                       const int* box, bool swizzle);
+                       const int* box, int swizzle_bytes);
 
 namespace {
 
@@ -46,7 +46,7 @@ constexpr float SA_RESCALE = 8.0f;   // log2 units
 int make_map(CUtensorMap* m, const void* base, const CacheAttn& a, int64_t S, int64_t H, int64_t B, const HeadStrides& st) {
   const int64_t dims[4] = {a.D, S, H, B}, strides[3] = {st.s, st.h, st.b};
   const int box[4] = {64, SA_KEYS, 1, 1};
-  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, true);
+  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, 128);
 }
 
 struct StreamArgs {

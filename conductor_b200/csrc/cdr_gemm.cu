@@ -566,9 +566,9 @@ int make_tensor_map_3d_plain(CUtensorMap* map, const void* base, int is_bf16, in
 }
 
 // 4-D tensor of 16-bit elements, extents dims[0..3] (dims[0] contiguous), element strides of dimensions
-// 1..3 (multiples of 8, in any order of size); swizzle 128 bytes or none.  Reads outside are zeros.
+// 1..3 (multiples of 8, in any order of size); swizzle of 128 or 64 bytes, or none (0).  Reads outside are zeros.
 int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const int64_t* dims, const int64_t* strides,
-                       const int* box, bool swizzle) {
+                       const int* box, int swizzle_bytes) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return CDR_ERR_CUDA; }
   cuuint64_t d[4], st[3];
@@ -577,8 +577,8 @@ int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const in
   for (int i = 0; i < 3; ++i) st[i] = static_cast<cuuint64_t>(strides[i]) * 2;
   CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  swizzle ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  swizzle_bytes == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled (4-D) failed with %d", static_cast<int>(r)); return CDR_ERR_CUDA; }
   return CDR_OK;
 }

@@ -28,7 +28,7 @@
 namespace cdr {
 
 int make_tensor_map_4d(CUtensorMap* map, const void* base, int is_bf16, const int64_t* dims, const int64_t* strides,
-                       const int* box, bool swizzle);
+                       const int* box, int swizzle_bytes);
 
 namespace {
 
@@ -58,11 +58,10 @@ struct TileSmem {
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int BAR_OFF = KV_OFF + KV_STAGES * TILE_BYTES;
-  static constexpr int STAGE_OFF = BAR_OFF + 256;
-  static constexpr int STAGE_BYTES = 8 * 32 * 64;              // 8 softmax warps x 32 rows x 32 16-bit columns
-  static constexpr int PART_STAGE_BYTES = 2 * STAGE_BYTES;     // PACKED: fp32 columns
-  static constexpr size_t TOTAL = STAGE_OFF + STAGE_BYTES + 1024;
-  static constexpr size_t TOTAL_PACKED = STAGE_OFF + PART_STAGE_BYTES + 1024;
+  static constexpr int STAGE_OFF = BAR_OFF + 1024;
+  // 8 softmax warps x two stages of 32 rows x 32 16-bit columns (PACKED: one of fp32 columns)
+  static constexpr int WARP_STAGE = 2 * 32 * 64;
+  static constexpr size_t TOTAL = STAGE_OFF + 8 * WARP_STAGE + 1024;
 };
 
 enum { B_QFULL = 0, B_QEMPTY = 1, B_FULL = 2, B_EMPTY = B_FULL + KV_STAGES, B_SFULL = B_EMPTY + KV_STAGES, B_PFULL = B_SFULL + 2,
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
     const uint32_t lane_sel = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t s_taddr = tmem_base + TMEM_S + g * 128 + lane_sel;
     const uint32_t o_taddr = tmem_base + TMEM_O + g * 128 + lane_sel;
-    unsigned char* stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * (32 * 64);
+    unsigned char* stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * L::WARP_STAGE;
     int n = 0;                                       // key blocks consumed so far over all tiles
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -427,6 +426,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const int row0 = r.q0 + g * HALF;
       const int p_first = r.off + row0, p_last = r.off + min(row0 + HALF, a.Sq) - 1;
       const int pos = p_first + row_in_half;         // this row's position (PACKED: unused)
+      const int warp_first = p_first + q * 32;       // and of the warp's first row
       // (selected, not indexed: an index that the compiler does not know would put the tile into local memory)
       const int live = g ? r.live[1] : r.live[0], light = g ? r.light[1] : r.light[0];
       const int pre = g ? r.pre[1] : r.pre[0], wa = g ? r.wa[1] : r.wa[0], wb = g ? r.wb[1] : r.wb[0];
@@ -468,18 +468,20 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
             const int see = pos - key0;              // visible: i <= see
 #pragma unroll
             for (int c = 0; c < 4; ++c)
+              if (key0 + c * 32 + 31 > warp_first)   // else every row of the warp sees the chunk
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c * 32 + i > see) sr[c][i] = __float_as_uint(-INFINITY);
+                for (int i = 0; i < 32; ++i)
+                  if (c * 32 + i > see) sr[c][i] = __float_as_uint(-INFINITY);
           }
           if (key0 <= p_last - a.window && key0 + BKV > a.sinks) {   // keys in front of some row's window
             const int gone = pos - a.window - key0;  // hidden: i <= gone, unless among the sinks
             if (key0 >= a.sinks) {
 #pragma unroll
               for (int c = 0; c < 4; ++c)
+                if (key0 + c * 32 <= warp_first + 31 - a.window)
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (c * 32 + i <= gone) sr[c][i] = __float_as_uint(-INFINITY);
+                  for (int i = 0; i < 32; ++i)
+                    if (c * 32 + i <= gone) sr[c][i] = __float_as_uint(-INFINITY);
             } else {
               const int sink = a.sinks - key0;
 #pragma unroll
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         const int half_rows = a.G * a.Sq * t.seqs_per_half;
         const int64_t at = (static_cast<int64_t>(r.off) * a.Hkv + r.hkv) * t.part_rows + (r.b / t.seqs_per_half + g) * HALF;
         if (row_in_half < half_rows) t.part_lse[at + row_in_half] = none ? -INFINITY : m_ref + __log2f(l);
-        unsigned char* part_stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * (32 * 128);
+        unsigned char* part_stage = stage;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
@@ -597,15 +599,17 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 #pragma unroll
             for (int x = 0; x < 16; ++x) w[x] = 0u;    // a half of padding: nothing was computed
           }
-          if (lane == 0) sm100::bulk_wait_read<0>();
+          // two stages in turn, 64-byte swizzled (the lanes' 64-byte rows would meet in four banks)
+          if (lane == 0) sm100::bulk_wait_read<1>();
           __syncwarp();
+          unsigned char* out = stage + (c & 1) * (32 * 64);
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + x * 16) = make_uint4(w[x * 4], w[x * 4 + 1], w[x * 4 + 2], w[x * 4 + 3]);
+            *reinterpret_cast<uint4*>(out + lane * 64 + ((x ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[x * 4], w[x * 4 + 1], w[x * 4 + 2], w[x * 4 + 3]);
           sm100::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            sm100::tma_store_4d(&t.tmap_o, stage, c * 32, row0 + q * 32, r.hq, r.b);
+            sm100::tma_store_4d(&t.tmap_o, out, c * 32, row0 + q * 32, r.hq, r.b);
             sm100::bulk_commit();
           }
         }
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 template <int HD, bool BF16, bool PACKED>
 int launch_tile_cfg(TileArgs& t, int64_t tiles, int ctas, void* counter, cudaStream_t stream) {
   auto kern = tile_attention_kernel<HD, BF16, PACKED>;
-  constexpr size_t smem = PACKED ? TileSmem<HD>::TOTAL_PACKED : TileSmem<HD>::TOTAL;
+  constexpr size_t smem = TileSmem<HD>::TOTAL;
   static bool configured_dev[64] = {false};
   int dev = 0;
   CDR_CUDA_TRY(cudaGetDevice(&dev));
@@ -671,10 +675,10 @@ int launch_tile_typed(TileArgs& t, int64_t tiles, int ctas, void* counter, cudaS
 }
 
 int map_heads(CUtensorMap* m, const void* base, const CacheAttn& a, int64_t S, int64_t H, int64_t B, const HeadStrides& st, int box_d,
-              int box_s, int box_h, int box_b, bool swizzle) {
+              int box_s, int box_h, int box_b, int swizzle_bytes) {
   const int64_t dims[4] = {a.D, S, H, B}, strides[3] = {st.s, st.h, st.b};
   const int box[4] = {box_d, box_s, box_h, box_b};
-  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, swizzle);
+  return make_tensor_map_4d(m, base, a.bf16, dims, strides, box, swizzle_bytes);
 }
 
 int map_prefix(TileArgs& t) {
@@ -682,8 +686,8 @@ int map_prefix(TileArgs& t) {
   if (a.P == 0) return CDR_OK;
   HeadStrides pk = a.spk, pv = a.spv;
   pk.b = pv.b = a.D;             // one "sequence": the stride is never used
-  if (int rc = map_heads(&t.tmap_pk, a.pk, a, a.P, a.Hkv, 1, pk, 64, BKV, 1, 1, true)) return rc;
-  return map_heads(&t.tmap_pv, a.pv, a, a.P, a.Hkv, 1, pv, 64, BKV, 1, 1, true);
+  if (int rc = map_heads(&t.tmap_pk, a.pk, a, a.P, a.Hkv, 1, pk, 64, BKV, 1, 1, 128)) return rc;
+  return map_heads(&t.tmap_pv, a.pv, a, a.P, a.Hkv, 1, pv, 64, BKV, 1, 1, 128);
 }
 
 }  // namespace
@@ -691,11 +695,11 @@ int map_prefix(TileArgs& t) {
 int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
   TileArgs t = {};
   t.a = a;
-  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, HALF, 1, 1, true)) return rc;
-  if (int rc = map_heads(&t.tmap_o, a.out, a, a.Sq, a.Hq, a.B, a.so, 32, 32, 1, 1, false)) return rc;
+  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, HALF, 1, 1, 128)) return rc;
+  if (int rc = map_heads(&t.tmap_o, a.out, a, a.Sq, a.Hq, a.B, a.so, 32, 32, 1, 1, 64)) return rc;
   if (a.Skv > 0) {               // an empty cache is never loaded from
-    if (int rc = map_heads(&t.tmap_k, a.k, a, a.Skv, a.Hkv, a.B, a.sk, 64, BKV, 1, 1, true)) return rc;
-    if (int rc = map_heads(&t.tmap_v, a.v, a, a.Skv, a.Hkv, a.B, a.sv, 64, BKV, 1, 1, true)) return rc;
+    if (int rc = map_heads(&t.tmap_k, a.k, a, a.Skv, a.Hkv, a.B, a.sk, 64, BKV, 1, 1, 128)) return rc;
+    if (int rc = map_heads(&t.tmap_v, a.v, a, a.Skv, a.Hkv, a.B, a.sv, 64, BKV, 1, 1, 128)) return rc;
   }
   if (int rc = map_prefix(t)) return rc;
   t.n_qtiles = (a.Sq + BQ - 1) / BQ;
@@ -767,7 +771,7 @@ int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cud
   t.part_rows = static_cast<int>(rows);
   t.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kTileCounterBytes);
   t.part_lse = t.part_o + static_cast<size_t>(t.splits) * a.Hkv * rows * a.D;
-  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, a.Sq, a.G, t.seqs_per_half, true)) return rc;
+  if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, a.Sq, a.G, t.seqs_per_half, 128)) return rc;
   if (int rc = map_prefix(t)) return rc;
   *part = PrefixPartials{t.part_o, t.part_lse, t.splits, t.part_rows, t.seqs_per_half};
   return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, plan.ctas, ws, stream);
