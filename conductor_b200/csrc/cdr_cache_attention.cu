@@ -39,7 +39,6 @@ namespace {
 
 constexpr int SA_ROWS = 16;          // query rows of a task (m of the matrix instruction)
 constexpr int SA_KEYS = 32;          // keys per unit
-constexpr int SA_STAGES = 2;         // units in flight per warp
 constexpr int SA_GROUPS = 2048;      // entries of the table of cumulated units
 constexpr float SA_RESCALE = 8.0f;   // log2 units
 
@@ -304,16 +303,18 @@ struct __align__(16) UnitHeader {
   int b, hkv, mt, off, task_first;
 };
 
-// 6 warps at HD = 128, 12 at HD = 64, where a unit has half the bytes and about as many dependent steps.
+// 192 KB in flight per SM either way; at HD = 64 a unit has half the bytes and about as many dependent steps (8 warps of
+// three units: 5.6 against 5.8 TB/s).
 template <int HD>
 struct StreamSmem {
   static constexpr int WARPS = HD == 128 ? 6 : 12;
+  static constexpr int STAGES = 2;                                        // units in flight per warp
   static constexpr int THREADS = WARPS * 32;
   static constexpr int HALF_BYTES = SA_KEYS * HD * 2;          // K or V of a unit
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-  static constexpr int HEAD_OFF = WARPS * SA_STAGES * STAGE_BYTES;
-  static constexpr int BAR_OFF = HEAD_OFF + WARPS * SA_STAGES * static_cast<int>(sizeof(UnitHeader));
-  static constexpr int CUM_OFF = BAR_OFF + WARPS * SA_STAGES * 8;
+  static constexpr int HEAD_OFF = WARPS * STAGES * STAGE_BYTES;
+  static constexpr int BAR_OFF = HEAD_OFF + WARPS * STAGES * static_cast<int>(sizeof(UnitHeader));
+  static constexpr int CUM_OFF = BAR_OFF + WARPS * STAGES * 8;
   static constexpr int FIXED = CUM_OFF + 1024;                 // alignment slack
 };
 
@@ -330,12 +331,12 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
   const CacheAttn& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  UnitHeader* heads = reinterpret_cast<UnitHeader*>(smem + L::HEAD_OFF) + warp * SA_STAGES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF) + warp * SA_STAGES;
-  unsigned char* ring = smem + warp * (SA_STAGES * L::STAGE_BYTES);
+  UnitHeader* heads = reinterpret_cast<UnitHeader*>(smem + L::HEAD_OFF) + warp * L::STAGES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF) + warp * L::STAGES;
+  unsigned char* ring = smem + warp * (L::STAGES * L::STAGE_BYTES);
   if (lane == 0) {
     if (a.Skv > 0) { sm100::prefetch_tensormap(&args.tmap_k); sm100::prefetch_tensormap(&args.tmap_v); }
-    for (int st = 0; st < SA_STAGES; ++st) sm100::mbar_init(&bars[st], 1);
+    for (int st = 0; st < L::STAGES; ++st) sm100::mbar_init(&bars[st], 1);
     sm100::fence_barrier_init();
   }
   __syncwarp();
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
     ++lu;
   };
 #pragma unroll
-  for (int st = 0; st < SA_STAGES; ++st) load_unit(st);
+  for (int st = 0; st < L::STAGES; ++st) load_unit(st);
   __syncwarp();
 
   uint4 qf[2][AC][2];
@@ -465,12 +466,8 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
           mma16816<BF16>(s[n], qf[0][j][y].z, qf[1][j][y].z, qf[0][j][y].w, qf[1][j][y].w, kf.z, kf.w);
         }
 
-    // scores in log2 units; s[n][2x + e] belongs to row g + 8x and key base + 8n + 2c + e
+    // s[n][2x + e] belongs to row g + 8x and key base + 8n + 2c + e
     const bool own = h.flags & 1, partial = h.base + SA_KEYS > h.end;
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] *= a.scale_log2;
     if (own || partial) {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
@@ -486,7 +483,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
       float v = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
                       fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
       v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-      mx[x] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+      mx[x] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)) * a.scale_log2;     // scale > 0: the maximum commutes with it
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] + SA_RESCALE || mx[1] > m[1] + SA_RESCALE)) {
 #pragma unroll
@@ -508,7 +505,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float p = ex2(s[n][2 * x + e] - ref);
+          const float p = ex2(fmaf(s[n][2 * x + e], a.scale_log2, -ref));
           s[n][2 * x + e] = p;
           l[x] += p;
         }
@@ -538,7 +535,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
     __syncwarp();                                // every lane is done with the stage and its header
     load_unit(st);
     __syncwarp();
-    if (++st == SA_STAGES) { st = 0; phase ^= 1; }
+    if (++st == L::STAGES) { st = 0; phase ^= 1; }
 
     if (!CLUSTER && (h.flags & 4)) {
       // ---- end of a segment: o[j][e][2x + i] is row g + 8x, column 64 j + 8 (2c + i) + e
@@ -626,7 +623,7 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
         sum.join_parts(sub, tpp, n_parts, [&](int n, const float** o) {
           const int wn = n % L::WARPS, cn = n / L::WARPS;
           const float2* pml = &sm_ml[wn][row];
-          *o = reinterpret_cast<const float*>(smem + wn * (SA_STAGES * L::STAGE_BYTES)) + row * PITCH + d;
+          *o = reinterpret_cast<const float*>(smem + wn * (L::STAGES * L::STAGE_BYTES)) + row * PITCH + d;
           if (cs > 1) {
             pml = static_cast<const float2*>(__cluster_map_shared_rank(pml, cn));
             *o = static_cast<const float*>(__cluster_map_shared_rank(*o, cn));
@@ -748,6 +745,8 @@ StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
   if (p.tasks <= sms) {
     p.cluster = 1;
     while (p.cluster < 8 && p.tasks * p.cluster * 2 <= sms && per_head > p.m_tiles * p.cluster * warps) p.cluster *= 2;
+    // long shares: the list fills all SMs and reads 6 TB/s, clusters of 128 CTAs 4 (2 sequences of 131072 keys: 267 us so)
+    if (per_head > 8LL * p.m_tiles * p.cluster * warps) p.cluster = 0;
   }
   // every warp the machine can hold at once, if there is a unit for each
   p.ctas = static_cast<int>(p.units < sms ? (p.units < 1 ? 1 : p.units) : sms);
