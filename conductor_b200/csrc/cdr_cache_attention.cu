@@ -722,29 +722,27 @@ __global__ void __launch_bounds__(CA_THREADS) combine_parts_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------- host side
-struct StreamPlan {
-  int m_tiles, ctas, n_warps, rows_cap, group, groups;
-  int cluster;                     // > 0: a cluster of so many CTAs per task, no scratch
-  int64_t tasks, slots, units;     // units: the most there can be (every sequence at full length)
-};
+// Clusters of 2, 4, 8 CTAs that the current device holds at once (a GPC of 16 or 18 SMs does not always take two of eight).
+int max_clusters(int D, int size);
 
-StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
+// `packed`: behind the packed prefix product, on the SMs that it leaves
+StreamPlan plan_stream(const CacheAttn& a, const PackedPlan* packed) {
   StreamPlan p;
   const int warps = a.D == 128 ? StreamSmem<128>::WARPS : StreamSmem<64>::WARPS;
   const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
   p.m_tiles = static_cast<int>((rows + SA_ROWS - 1) / SA_ROWS);
   p.rows_cap = static_cast<int>(rows < SA_ROWS ? rows : SA_ROWS);
   p.tasks = static_cast<int64_t>(a.B) * a.Hkv * p.m_tiles;
-  const int prefix = behind_prefix ? 0 : a.P;
+  const int prefix = packed ? 0 : a.P;
   int64_t per_head = 0;
   for (int mt = 0; mt < p.m_tiles; ++mt) per_head += key_ranges(a, prefix, a.Skv, mt).n_total;
   p.units = per_head * a.B * a.Hkv;
-  // (behind the packed product: on the SMs that it leaves)
-  const int64_t sms = behind_prefix ? (sm_count() > packed_ctas(a) ? sm_count() - packed_ctas(a) : 1) : sm_count();
+  const int64_t sms = packed ? (sm_count() > packed->ctas ? sm_count() - packed->ctas : 1) : sm_count();
   p.cluster = 0;
   if (p.tasks <= sms) {
     p.cluster = 1;
-    while (p.cluster < 8 && p.tasks * p.cluster * 2 <= sms && per_head > p.m_tiles * p.cluster * warps) p.cluster *= 2;
+    while (p.cluster < 8 && p.tasks * p.cluster * 2 <= sms && per_head > p.m_tiles * p.cluster * warps && p.tasks <= max_clusters(a.D, p.cluster * 2))
+      p.cluster *= 2;
     // long shares: the list fills all SMs and reads 6 TB/s, clusters of 128 CTAs 4 (2 sequences of 131072 keys: 267 us so)
     if (per_head > 8LL * p.m_tiles * p.cluster * warps) p.cluster = 0;
   }
@@ -753,7 +751,7 @@ StreamPlan plan_stream(const CacheAttn& a, bool behind_prefix) {
   p.n_warps = p.ctas * warps;
   p.group = (a.B + SA_GROUPS - 1) / SA_GROUPS;
   p.groups = (a.B + p.group - 1) / p.group;
-  p.slots = p.cluster ? 0 : 2LL * p.n_warps + (behind_prefix ? p.tasks : 0);
+  p.slots = p.cluster ? 0 : 2LL * p.n_warps + (packed ? p.tasks : 0);
   return p;
 }
 
@@ -763,17 +761,53 @@ size_t stream_bytes(const CacheAttn& a, const StreamPlan& p) {
   return p.cluster ? 0 : table_bytes(p) + static_cast<size_t>(p.slots) * p.rows_cap * (a.D + 2) * sizeof(float);
 }
 
+template <int HD, bool BF16, bool CLUSTER>
+cudaError_t configure_stream() {
+  constexpr int most = StreamSmem<HD>::FIXED + SA_GROUPS * static_cast<int>(sizeof(int));
+  return cudaFuncSetAttribute(stream_attention_kernel<HD, BF16, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+}
+
+template <int HD>
+int query_clusters(int size) {
+  if (configure_stream<HD, true, true>() != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(size), 1, 1);
+  cfg.blockDim = dim3(StreamSmem<HD>::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = StreamSmem<HD>::FIXED;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, stream_attention_kernel<HD, true, true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+int max_clusters(int D, int size) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  static int known[64][2][4] = {};             // count + 1; a race stores the same value twice
+  int& k = known[dev][D == 128][size == 2 ? 1 : size == 4 ? 2 : 3];
+  if (k == 0) k = 1 + (D == 128 ? query_clusters<128>(size) : query_clusters<64>(size));
+  return k - 1;
+}
+
 template <int HD, bool BF16>
 int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStream_t stream) {
   using L = StreamSmem<HD>;
-  constexpr int most = L::FIXED + SA_GROUPS * static_cast<int>(sizeof(int));
   const size_t table = s.a.lengths && !p.cluster ? s.groups * sizeof(int) : 0;
   int dev = 0;
   CDR_CUDA_TRY(cudaGetDevice(&dev));
   static bool configured_dev[64] = {false};
   if (!configured_dev[dev & 63]) {
-    CDR_CUDA_TRY(cudaFuncSetAttribute(stream_attention_kernel<HD, BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    CDR_CUDA_TRY(cudaFuncSetAttribute(stream_attention_kernel<HD, BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    CDR_CUDA_TRY((configure_stream<HD, BF16, false>()));
+    CDR_CUDA_TRY((configure_stream<HD, BF16, true>()));
     configured_dev[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -807,12 +841,9 @@ int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStr
 
 }  // namespace
 
-float stream_units(const CacheAttn& a) { return static_cast<float>(a.B) * a.Hkv * head_units(a, 0, a.Skv, static_cast<int>((static_cast<int64_t>(a.G) * a.Sq + SA_ROWS - 1) / SA_ROWS)); }
+namespace {
 
-size_t stream_workspace(const CacheAttn& a, bool behind_prefix) { return stream_bytes(a, plan_stream(a, behind_prefix)); }
-
-int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void* ws, cudaStream_t stream) {
-  const StreamPlan p = plan_stream(a, part.splits > 0);
+int launch_stream_attention(const CacheAttn& a, const StreamPlan& p, const PrefixPartials& part, void* ws, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
   if (p.units > 0x3fffffff || p.tasks > 0x3fffffff || rows > 0x3fffffff) { set_error("attention: too many row tiles for one launch"); return CDR_ERR_UNSUPPORTED; }
   StreamArgs s = {};
@@ -846,7 +877,6 @@ int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void
 }
 
 // ---------------------------------------------------------------- entry points
-namespace {
 
 // [.., S, D] operand: D contiguous, every other stride a positive multiple of 16 bytes.  Extents of 1
 // get a stride that the kernels may use for address arithmetic.
@@ -969,41 +999,67 @@ int parse_prefix(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_
   return CDR_OK;
 }
 
-// Which kernels a call runs.
+// Which kernels a call runs, and their scratch.
 enum class Path { kStream, kTile, kPacked };
 
-Path choose_path(const CacheAttn& a) {
-  if (a.Sq >= 64) return Path::kTile;
-  const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
-  if (a.P >= 128 && rows <= 128 && a.B * rows > 32) return Path::kPacked;
-  return Path::kStream;
-}
+struct CachePlan {
+  Path path;
+  PackedPlan packed;
+  StreamPlan stream;
+  size_t packed_bytes, bytes;      // of the product's part of the scratch, of all
+};
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t cache_attention_workspace(const CacheAttn& a) {
-  switch (choose_path(a)) {
-    case Path::kTile: return kTileCounterBytes;
-    case Path::kPacked: return round256(packed_workspace(a)) + stream_workspace(a, true);
-    default: return stream_workspace(a, false);
+// By estimated times in us (B200).  Streaming: 6 per call and, per unit of 32 keys that a warp takes in turn, 1.7 where the rows
+// of a task share one position and 2.8 where they do not.  Tiles: 6 and 2.0 per round of 128-key blocks.  Measured:
+// 8 sequences, 32 / 8 heads, 4096 keys: 16 queries 97 streamed / 128 in tiles, 24 queries 144 / 128; 1 sequence: 48 queries
+// 49 / 63.  Prefix of 4096 keys, 8 heads, 64 own keys: 4 sequences 14 streamed / 18 packed, 8 sequences 24 / 18, 64 118 / 21;
+// of 16384: 2 sequences 24 / 29, 4 sequences 37 / 33.
+CachePlan plan_call(const CacheAttn& a) {
+  CachePlan c;
+  c.packed_bytes = 0;
+  if (a.Sq >= 256) {
+    c.path = Path::kTile;
+    c.bytes = kTileCounterBytes;
+    return c;
   }
+  const int warps = sm_count() * (a.D == 128 ? StreamSmem<128>::WARPS : StreamSmem<64>::WARPS);
+  const float unit_us = a.Sq == 1 ? 1.7f : 2.8f;
+  c.stream = plan_stream(a, nullptr);
+  const float stream_us = 6.0f + c.stream.units * unit_us / warps;
+  const float tile_us = tile_attention_us(a);
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Sq;
+  if (a.P >= 128 && rows <= 128 && a.B > 1) {
+    const PackedPlan packed = plan_packed(a, c.stream.units - static_cast<int64_t>(c.stream.tasks) * ((a.P + SA_KEYS - 1) / SA_KEYS));
+    if (packed.us < stream_us && packed.us < tile_us) {
+      c.path = Path::kPacked;
+      c.packed = packed;
+      c.stream = plan_stream(a, &packed);
+      c.packed_bytes = round256(packed_workspace(a, packed));
+      c.bytes = c.packed_bytes + stream_bytes(a, c.stream);
+      return c;
+    }
+  }
+  c.path = tile_us < stream_us ? Path::kTile : Path::kStream;
+  c.bytes = c.path == Path::kTile ? kTileCounterBytes : stream_bytes(a, c.stream);
+  return c;
 }
 
 int run_cache_attention(const CacheAttn& a, const char* op, void* ws, size_t ws_bytes, cudaStream_t stream) {
-  const Path path = choose_path(a);
-  const size_t need = cache_attention_workspace(a);
-  if (need && (!ws || ws_bytes < need)) {
-    set_error("%s: workspace of %zu bytes required, got %zu", op, need, ws ? ws_bytes : (size_t)0);
+  const CachePlan c = plan_call(a);
+  if (c.bytes && (!ws || ws_bytes < c.bytes)) {
+    set_error("%s: workspace of %zu bytes required, got %zu", op, c.bytes, ws ? ws_bytes : (size_t)0);
     return CDR_ERR_WORKSPACE;
   }
-  if (need && (reinterpret_cast<uintptr_t>(ws) & 31u)) { set_error("%s: workspace must be 32-byte aligned", op); return CDR_ERR_MISALIGNED; }
+  if (c.bytes && (reinterpret_cast<uintptr_t>(ws) & 31u)) { set_error("%s: workspace must be 32-byte aligned", op); return CDR_ERR_MISALIGNED; }
+  if (c.path == Path::kTile) return launch_tile_attention(a, ws, stream);
   PrefixPartials part{nullptr, nullptr, 0, 0, 1};
-  if (path == Path::kTile) return launch_tile_attention(a, ws, stream);
-  if (path == Path::kPacked) {
-    if (int rc = launch_packed_prefix(a, ws, &part, stream)) return rc;
-    ws = static_cast<unsigned char*>(ws) + round256(packed_workspace(a));
+  if (c.path == Path::kPacked) {
+    if (int rc = launch_packed_prefix(a, c.packed, ws, &part, stream)) return rc;
+    ws = static_cast<unsigned char*>(ws) + c.packed_bytes;
   }
-  return launch_stream_attention(a, part, ws, stream);
+  return launch_stream_attention(a, c.stream, part, ws, stream);
 }
 
 }  // namespace
@@ -1014,7 +1070,7 @@ int window_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor
   bool empty = false;
   *bytes = 0;
   if (int rc = parse_window(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
-  if (!empty) *bytes = cache_attention_workspace(a);
+  if (!empty) *bytes = plan_call(a).bytes;
   return CDR_OK;
 }
 
@@ -1024,7 +1080,7 @@ int prefix_attention_workspace(const cdr_tensor* ins, int n_in, const cdr_tensor
   bool empty = false;
   *bytes = 0;
   if (int rc = parse_prefix(ins, n_in, outs, n_out, p, &a, &empty)) return rc;
-  if (!empty) *bytes = cache_attention_workspace(a);
+  if (!empty) *bytes = plan_call(a).bytes;
   return CDR_OK;
 }
 

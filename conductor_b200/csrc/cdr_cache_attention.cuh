@@ -50,20 +50,30 @@ struct PrefixPartials {
   }
 };
 
-// Few query rows per key head: the keys are streamed once (cdr_cache_attention.cu).  part.splits > 0: joined with
-// the partial results (launched right behind the kernel that makes them); else the prefix is streamed as well.
-int launch_stream_attention(const CacheAttn& a, const PrefixPartials& part, void* ws, cudaStream_t stream);
-size_t stream_workspace(const CacheAttn& a, bool behind_prefix);   // 16-byte aligned start
-float stream_units(const CacheAttn& a);        // 16 KB (D = 128) pieces of own keys, at full lengths
+// How the packed product over the shared prefix is cut (cdr_tile_attention.cu).
+struct PackedPlan {
+  int seqs_per_half, row_tiles, split_blocks, splits;
+  int ctas;            // SMs it takes; the streaming kernel behind it runs on the others
+  float us;            // estimated time of both
+};
 
-// Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter.
+// How the keys of few query rows are streamed (cdr_cache_attention.cu).
+struct StreamPlan {
+  int m_tiles, ctas, n_warps, rows_cap, group, groups;
+  int cluster;         // > 0: a cluster of so many CTAs per task, no scratch
+  int64_t tasks, slots, units;     // units of 32 keys: the most there can be (every sequence at full length)
+};
+
+// Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter, 32-byte aligned.
 constexpr size_t kTileCounterBytes = 256;
 // prefix, sinks and window of every (sequence, query head), 256 queries per tile
 int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream);
-// the shared prefix alone, for G * Sq <= 128 query rows per sequence and key head, into *part in `ws`
-int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream);
-size_t packed_workspace(const CacheAttn& a);   // with the counter; 32-byte aligned start
-int packed_ctas(const CacheAttn& a);           // SMs it takes; the streaming kernel behind it runs on the others
+float tile_attention_us(const CacheAttn& a);   // estimated time
+// the shared prefix alone, for G * Sq <= 128 query rows per sequence and key head, into *part in `ws`; `own_units`: of the
+// streaming kernel that runs beside it
+PackedPlan plan_packed(const CacheAttn& a, int64_t own_units);
+size_t packed_workspace(const CacheAttn& a, const PackedPlan& plan);   // with the counter
+int launch_packed_prefix(const CacheAttn& a, const PackedPlan& plan, void* ws, PrefixPartials* part, cudaStream_t stream);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ int sequence_length(const CacheAttn& a, int b) {

@@ -692,6 +692,13 @@ int map_prefix(TileArgs& t) {
 
 }  // namespace
 
+float tile_attention_us(const CacheAttn& a) {
+  const int64_t keys = static_cast<int64_t>(a.window) + (a.Sq < BQ ? a.Sq : BQ);
+  const int64_t blocks = ((keys < a.Skv ? keys : a.Skv) + 2 * BKV - 1) / BKV + (a.P + BKV - 1) / BKV;
+  const int64_t tiles = static_cast<int64_t>(a.B) * a.Hq * ((a.Sq + BQ - 1) / BQ);
+  return 6.0f + (a.D == 128 ? 2.0f : 1.7f) * ((tiles + sm_count() - 1) / sm_count()) * blocks;
+}
+
 int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
   TileArgs t = {};
   t.a = a;
@@ -713,13 +720,9 @@ int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream) {
 // How the shared prefix is cut for the packed product, and how many CTAs it gets: the others of the machine's
 // SMs are left to the streaming kernel, which starts beside it (own keys from HBM under the product's arithmetic).
 // Both times are estimated, in us, from what the kernels measure on this machine: here 1.95 per block of 128 keys and 256
-// rows (1.6 with one live half), 3 per tile and 5 per launch; there 0.19 per 16 KB and SM, 8 per launch.  64 sequences of 32
+// rows (1.6 with one live half, a fifth less at D = 64), 3 per tile and 5 per launch; there 0.19 per 16 KB and SM, 8 per launch.  64 sequences of 32
 // heads behind 16384 keys, 512 own ones: 71 us one after the other, 46.6 with 88 CTAs here, 52.9 with 112, 72 with 120.
-struct PackedPlan {
-  int seqs_per_half, row_tiles, split_blocks, splits, ctas;
-};
-
-PackedPlan plan_packed(const CacheAttn& a) {
+PackedPlan plan_packed(const CacheAttn& a, int64_t own_units) {
   PackedPlan p;
   const int per_seq = a.G * a.Sq;
   const int fit = HALF / per_seq;
@@ -728,8 +731,8 @@ PackedPlan plan_packed(const CacheAttn& a) {
   const int blocks = (a.P + BKV - 1) / BKV;
   const int64_t tasks = static_cast<int64_t>(a.Hkv) * p.row_tiles;
   const int sms = sm_count();
-  const float per_block = p.seqs_per_half < a.B ? 1.95f : 1.6f;
-  const float stream_us = 0.19f * stream_units(a) * a.D / 128;
+  const float per_block = (p.seqs_per_half < a.B ? 1.95f : 1.6f) * (a.D == 128 ? 1.0f : 0.8f);
+  const float stream_us = 0.19f * own_units * a.D / 128;
   float best = INFINITY;
   for (int eighth = 4; eighth <= 8; ++eighth) {
     const int ctas = ((eighth == 8 ? sms - sms / 16 : sms * eighth / 8) + 3) / 4 * 4;
@@ -748,20 +751,17 @@ PackedPlan plan_packed(const CacheAttn& a) {
       }
     }
   }
+  p.us = best + 6.0f;            // and the parts are added up
   return p;
 }
 
-int packed_ctas(const CacheAttn& a) { return plan_packed(a).ctas; }
-
-size_t packed_workspace(const CacheAttn& a) {
-  const PackedPlan p = plan_packed(a);
+size_t packed_workspace(const CacheAttn& a, const PackedPlan& p) {
   return kTileCounterBytes + static_cast<size_t>(p.splits) * a.Hkv * p.row_tiles * 2 * HALF * (a.D + 1) * sizeof(float);
 }
 
-int launch_packed_prefix(const CacheAttn& a, void* ws, PrefixPartials* part, cudaStream_t stream) {
+int launch_packed_prefix(const CacheAttn& a, const PackedPlan& plan, void* ws, PrefixPartials* part, cudaStream_t stream) {
   TileArgs t = {};
   t.a = a;
-  const PackedPlan plan = plan_packed(a);
   t.seqs_per_half = plan.seqs_per_half;
   t.n_qtiles = plan.row_tiles;
   t.split_blocks = plan.split_blocks;

@@ -103,7 +103,7 @@ def test_masked_scores_of_the_lowest_value_and_large_scores(Sq, Skv):
         check(WINDOW(q, kk, v, 9999, 0, scale=0.9), reference(q, kk, v, window=9999, scale=0.9))
 
 
-@pytest.mark.parametrize("Sq", [1, 3, 200])
+@pytest.mark.parametrize("Sq", [1, 3, 200, 300])
 def test_views_are_read_in_place(Sq):
     B, Hq, Hkv, Skv, D = 2, 8, 2, 333, 64
     q, k, v = cache(B, Hq, Hkv, Sq, Skv, D)
