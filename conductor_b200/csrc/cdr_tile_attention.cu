@@ -14,9 +14,19 @@
 //     to the other warps with the tile index.  Masks are applied on the blocks at the edges only.
 //   - the cache behind L may hold anything: its scores are masked, and its V rows, which would turn a
 //     zero weight into NaN, are cleared in shared memory by the MMA warp (last block of a sequence only).
+//   - a first block that holds nothing but up to 32 sinks is cut to 32 keys (two k-steps of P V, 32 columns of softmax):
+//     with a window of 512 keys it would else be a sixth of the work (8 x 2048 prompt, 128 -> 122 us).
 //   - PACKED (shared prefix): the 128 rows of a half are the G*Sq rows of several sequences that share a key
 //     head, fetched by one 4-D box; the prefix is split over tiles and O / l and log2 of the sum go to
 //     scratch in fp32, where the streaming kernel joins them with the sequences' own keys.
+// What bounds it: the chain softmax -> own products -> softmax of a half, and the MMA warp, which is busy for 2950 of
+// the 3770 cycles of a block pair (2070 of them are matrix time, the rest barriers, commits and hand-overs).  Measured
+// (B200): 4 x 1024 queries behind 4096 shared keys 167 us, 0.92 PFLOP/s of 1.60 that a large library product reaches; an
+// 8192 prompt with a window of 2048 267 us, 0.90; 8 x 2048 with a window of 512 117 us, 0.52 (masked halves of edge
+// blocks, and an epilogue every 5 blocks).
+// Measured and dropped: products cut to the visible keys in every edge block (operand shapes that the issuing warp computes
+// at run time cost it 20 %, 172 -> 205 us on the first case); edge blocks by 32-column chunks that are skipped, masked or
+// plain (2700 cycles per block, unrolled or as a loop, against 2500 for masking the whole score row).
 #include <cuda.h>
 #include <math.h>
 
@@ -195,7 +205,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0 && lane == 0) {
     sm100::prefetch_tensormap(&t.tmap_q);
-    if (!PACKED) { sm100::prefetch_tensormap(&t.tmap_k); sm100::prefetch_tensormap(&t.tmap_v); sm100::prefetch_tensormap(&t.tmap_o); }
+    if (!PACKED) sm100::prefetch_tensormap(&t.tmap_o);
+    if (!PACKED && a.Skv > 0) { sm100::prefetch_tensormap(&t.tmap_k); sm100::prefetch_tensormap(&t.tmap_v); }
     if (a.P > 0) { sm100::prefetch_tensormap(&t.tmap_pk); sm100::prefetch_tensormap(&t.tmap_pv); }
     for (int i = 0; i < B_COUNT; ++i) {
       const bool per_warp = (i >= B_PFULL && i < B_PFULL + 2) || (i >= B_OFREE && i < B_OFREE + 2);

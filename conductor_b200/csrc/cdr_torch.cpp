@@ -38,6 +38,11 @@ struct CallState {
   LaunchMany launch = nullptr;
 };
 
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 struct CallObject {
   PyObject_HEAD
   CallState* state;
@@ -97,17 +102,22 @@ PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     if (e.aligned && (reinterpret_cast<uintptr_t>(p) & 15u)) Py_RETURN_NONE;
     st.in_desc[i].data = p;
   }
-  const c10::Device device = st.ins[0].device;
-  c10::cuda::OptionalCUDAGuard guard;
-  if (c10::cuda::current_device() != device.index()) guard.set_device(device);
-  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  at::Tensor out = at::empty(st.out_sizes, at::TensorOptions().dtype(st.ins[0].dtype).device(device));
-  st.out_desc->data = out.data_ptr();
-  // scratch of this call alone: it goes back to the stream's pool once the launch is enqueued
-  void* ws = st.item->workspace_bytes ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(st.item->workspace_bytes, stream) : nullptr;
-  st.item->workspace = ws;
-  const int rc = st.launch(st.item, 1, stream, nullptr);
-  if (ws) c10::cuda::CUDACachingAllocator::raw_delete(ws);
+  at::Tensor out;
+  int rc = 0;
+  {
+    NoGil no_gil;                 // a full launch queue must not keep other threads from Python
+    const c10::Device device = st.ins[0].device;
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != device.index()) guard.set_device(device);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    out = at::empty(st.out_sizes, at::TensorOptions().dtype(st.ins[0].dtype).device(device));
+    st.out_desc->data = out.data_ptr();
+    // scratch of this call alone: it goes back to the stream's pool once the launch is enqueued
+    void* ws = st.item->workspace_bytes ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(st.item->workspace_bytes, stream) : nullptr;
+    st.item->workspace = ws;
+    rc = st.launch(st.item, 1, stream, nullptr);
+    if (ws) c10::cuda::CUDACachingAllocator::raw_delete(ws);
+  }
   if (rc != 0) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

@@ -18,7 +18,9 @@ place when ``D`` is contiguous and the other strides are multiples of 8 elements
 gathered first.  ``lengths`` (``[B]``, int32 or int64, on the same device) is how many keys each
 sequence uses, clamped to ``0 .. Skv``; what the cache holds behind them does not matter.  Query ``i`` stands
 at position ``p = L - Sq + i``; a query with ``p < 0`` sees nothing, and a query that sees nothing
-returns 0.  ``scale`` defaults to ``1 / sqrt(D)``.  The result is contiguous ``[B, Hq, Sq, D]``.
+returns 0.  ``scale`` defaults to ``1 / sqrt(D)`` and is positive.  The result is contiguous ``[B, Hq, Sq, D]``.
+Among the keys in use, a non-finite value of ``k`` or ``v`` that some queries see and others do not may reach the others too
+(0 times infinity); with ``Sq = 1`` hidden keys may hold anything.
 """
 from __future__ import annotations
 
@@ -115,6 +117,8 @@ def _run(name, build, params, tensors):
 
 def _other_run(name, build, params, tensors):
     """A call that is not the last one of its parameters again: found among the kept ones, or made."""
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise ExecutionError(f"{name}: expected tensors, got {[type(t).__name__ for t in tensors]}", kernel_name=name)
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")

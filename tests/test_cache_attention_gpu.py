@@ -1,12 +1,16 @@
 """window_attention and prefix_attention on a GPU against their definition in 64 bits."""
 import ctypes
+import threading
 
 import pytest
 import torch
 
 import conductor
+from abi_util import execute_host, launch, workspace_bytes
 from cache_attention_ref import check, reference
 from conductor.compiler.loader import load_library
+from conductor_b200.codegen.kernel_templates import CdrWindowAttnParams
+from conductor_b200.codegen.operator_registry import Template
 from conductor.utils.exceptions import DeviceError, ExecutionError, UnsupportedOperationError
 
 pytestmark = pytest.mark.gpu
@@ -124,6 +128,38 @@ def test_views_are_read_in_place(Sq):
     check(PREFIX(token_major[0], pre, pre, *token_major[1:]), reference(q, k, v, prefix=(pre, pre)), "prefix")
 
 
+@pytest.mark.parametrize("B,Sq,Skv,P", [(1, 1, 3000, 0), (70, 1, 900, 0), (2, 300, 500, 0), (40, 1, 200, 1500)])
+def test_nan_in_a_query_stays_in_its_row(B, Sq, Skv, P):
+    q, k, v = cache(B, 8, 2, Sq, Skv, 64)
+    pre = [rand(2, P, 64, seed=50 + i) for i in range(2)]
+    call = (lambda q: PREFIX(q, *pre, k, v)) if P else (lambda q: WINDOW(q, k, v, 1 << 20))
+    clean = call(q)
+    broken = q.clone()
+    broken[B // 2, 3, Sq // 2, 5] = float("nan")
+    got = call(broken)
+    assert got[B // 2, 3, Sq // 2].isnan().all()
+    got[B // 2, 3, Sq // 2] = clean[B // 2, 3, Sq // 2]
+    assert torch.equal(got, clean)
+
+
+def test_thousands_of_sequences():
+    """More sequences than the table of units has entries; lengths as a strided view and behind an odd offset."""
+    B = 5000
+    q, k, v = cache(B, 2, 1, 1, 40, 64)
+    n = (torch.arange(2 * B, device=DEV, dtype=torch.int32) * 7919) % 41
+    every_other, shifted = n[::2], n[1:B + 1]
+    assert not every_other.is_contiguous()
+    for lengths in (every_other, shifted):
+        got = WINDOW(q, k, v, 9, 2, lengths=lengths)
+        scores = torch.einsum("bhqd,bkd->bhqk", q.double(), k[:, 0].double()) / 8
+        key, last = torch.arange(40, device=DEV).view(1, 1, 1, 40), lengths.view(B, 1, 1, 1) - 1
+        seen = (key <= last) & ((key > last - 9) | (key < 2))
+        w = torch.softmax(scores.masked_fill(~seen, float("-inf")), -1).nan_to_num(0.0)
+        want = torch.einsum("bhqk,bkd->bhqd", w, v[:, 0].double())
+        bound = 2.0 ** -8 * (torch.einsum("bhqk,bkd->bhqd", w, v[:, 0].double().abs()) + want.abs()) * 1.02 + 1e-6
+        assert ((got.double() - want).abs() <= bound).all()
+
+
 def test_empty_calls():
     q, k, v = cache(2, 4, 2, 3, 0, 64)
     assert torch.equal(WINDOW(q, k, v, 5), torch.zeros_like(q))
@@ -131,6 +167,8 @@ def test_empty_calls():
     assert WINDOW(q[:, :, :0], k, v, 5).shape == (2, 4, 0, 64)
     pre = rand(2, 10, 64)
     assert torch.equal(PREFIX(q, pre, pre, k, v), torch.zeros_like(q))       # no own keys: every query is padding
+    q = rand(2, 4, 300, 64)
+    assert torch.equal(WINDOW(q, k, v, 5), torch.zeros_like(q)) and torch.equal(PREFIX(q, pre, pre, k, v), torch.zeros_like(q))
 
 
 def test_refusals():
@@ -228,6 +266,65 @@ def test_more_tiles_than_processors_in_a_graph():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, want) for _g, out in graphs)
+
+
+def test_calls_from_several_threads():
+    q, k, v = cache(4, 8, 2, 1, 600, 128)
+    want = WINDOW(q, k, v, 256, 4)
+    bad = []
+
+    def work(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(50):
+                if not torch.equal(WINDOW(q, k, v, 256, 4), want):
+                    bad.append((seed, i))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_captured_sequence_with_runs_in_flight():
+    """Runs of one plan on branches of one graph: each has its own scratch (tile counter, partial results)."""
+    from conductor_b200.compiler.gcu_backend import get_gcu_backend
+
+    torch._dynamo.reset()
+    get_gcu_backend().clear_cache()
+    sets = [tuple(cache(20, 8, 2, 300, 300, 64, seed=10 * i)) for i in range(4)]
+    f = torch.compile(lambda q, k, v: conductor.ops.window_attention(q, k, v, 100, 4) * 2.0, backend="gcu")
+    want = [f(*s).clone() for s in sets]
+    plan = list(get_gcu_backend()._compiled_functions.values())[-1]
+    seq = plan.capture_sequence(sets, lanes=2)
+    for _ in range(3):
+        seq.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o[0], w) for o, w in zip(seq.all_outputs, want))
+
+
+def test_library_calls_with_strided_output_and_host_tensors():
+    q, k, v = cache(2, 4, 2, 3, 90, 64)
+    n = lens(90, 41)
+    p = CdrWindowAttnParams(0.125, 1, 20, 2)
+    want = reference(q, k, v, window=20, sinks=2, lengths=n)
+    out = torch.full((2, 3, 4, 64 + 8), 7.0, dtype=q.dtype, device=DEV)
+    view = out[..., :64].transpose(1, 2)
+    ws = torch.empty(max(1, workspace_bytes(Template.WINDOW_ATTENTION, [q, k, v, n], [view], p)), dtype=torch.uint8, device=DEV)
+    launch(Template.WINDOW_ATTENTION, [q, k, v, n], [view], p, workspace=ws)
+    check(view, want)
+    assert (out[..., 64:] == 7.0).all()                       # what lies between the rows is left as it was
+    host = torch.empty(q.shape, dtype=q.dtype)
+    assert execute_host(Template.WINDOW_ATTENTION, [t.cpu() for t in (q, k, v, n)], [host], p) == 0
+    check(host.to(DEV), want)
+    long_q = rand(40, 8, 300, 64)
+    lk, lv = rand(40, 2, 300, 64, seed=1), rand(40, 2, 300, 64, seed=2)
+    p = CdrWindowAttnParams(0.125, 0, 64, 0)
+    assert launch(Template.WINDOW_ATTENTION, [long_q, lk, lv], [torch.empty_like(long_q)], p, check=False) == -6      # no workspace
+    assert launch(Template.WINDOW_ATTENTION, [long_q, lk, lv], [torch.empty_like(long_q)], p,
+                  workspace=torch.empty(4096, dtype=torch.uint8, device=DEV)[8:], check=False) == -3
 
 
 def test_the_same_call_gives_the_same_bits():
