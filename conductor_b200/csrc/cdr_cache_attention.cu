@@ -10,7 +10,7 @@
 // finish together.  Each warp runs the online-softmax recurrence on its own, without a barrier:
 //   - the TMA unit brings K and V of a unit into the warp's own two-stage ring (16 KB per stage at HD = 128,
 //     192 KB in flight per SM); copying them with per-thread 16-byte asynchronous copies instead was
-//     bound by instructions and shared-memory traffic at 4.1 TB/s (440 instructions per 16 keys).
+//     bound by instructions and shared-memory traffic (64 sequences below: 126 us, 3.7 TB/s).
 //   - the 16-byte pieces are operand registers of m16n8k16 matrix instructions as they are: the order of the
 //     contraction index is free as long as both operands use the same one, so a lane takes a piece of a K
 //     row (and of the Q row) for two k-steps; for P V it takes a piece of four V rows and pairs them with byte
@@ -23,10 +23,10 @@
 // second kernel, launched to overlap this one's tail, adds up each row's parts in a fixed order (no atomics:
 // the same call gives the same bits) and those of the shared prefix (cdr_tile_attention.cu).  Where there are
 // few tasks, a task belongs to one thread-block cluster instead, whose warps join their parts through
-// distributed shared memory: one launch, no scratch (one sequence: 11.2 -> 8.8 us).
+// distributed shared memory: one launch, no scratch (one sequence: 11.2 -> 8.7 us).
 // P is rounded to the input type for the second product (relative 2^-8 at most per weight at bf16, independent per
 // key); scores, maxima, sums and O stay in fp32.
-// Measured (B200): 64 sequences of up to 4096 keys, 32 / 8 heads, window 2048: 84 us, 5.5 TB/s of 465 MB with both
+// Measured (B200): 64 sequences of up to 4096 keys, 32 / 8 heads, window 2048: 85 us, 5.5 TB/s of 465 MB with both
 // kernels; long caches (64 x 4096 keys, 2 x 131072) 6.2 TB/s, of 6.5 that a plain copy reaches.  Shorter calls are
 // bound by the latency of two dependent launches or of the cluster's exchange.
 #include <cuda.h>
@@ -873,8 +873,9 @@ int launch_stream_attention(const CacheAttn& a, const StreamPlan& p, const Prefi
   s.group = p.group;
   s.groups = p.groups;
   s.rows_cap = p.rows_cap;
-  // threads per row of the second kernel: by the parts a row may have (a CTA per row pays only where there are few rows:
-  // 2048 rows of 24 parts take 26 us so, 12 with two warps per row)
+  // threads per row of the second kernel, by the parts that a row may have; a CTA per row pays only where there are few
+  // rows.  Whole calls with 32 / 64 / 256 threads, us: 32 rows (131072 keys) 113 / 102 / 94, 64 rows (16384 keys) 43 / 37 / 32;
+  // 2048 rows behind a prefix of 65536 keys 97 / 94 / 109; 8192 rows behind 32768 keys, few parts, 180 / 192 / 232.
   const int64_t per_task = p.tasks ? p.units / p.tasks : 0, per_warp = p.units / p.n_warps + 1;
   const int64_t parts = per_task / per_warp + 1 + part.splits;
   const int tpr = rows <= 2 * sm_count() && parts > 16 ? 256 : parts <= 8 ? 32 : 64;

@@ -19,14 +19,14 @@
 //   - PACKED (shared prefix): the 128 rows of a half are the G*Sq rows of several sequences that share a key
 //     head, fetched by one 4-D box; the prefix is split over tiles and O / l and log2 of the sum go to
 //     scratch in fp32, where the streaming kernel joins them with the sequences' own keys.
-// What bounds it: the chain softmax -> own products -> softmax of a half, and the MMA warp, which is busy for 2950 of
-// the 3770 cycles of a block pair (2070 of them are matrix time, the rest barriers, commits and hand-overs).  Measured
+// What bounds it: the chain softmax -> own products -> softmax of a half, and the MMA warp, which in a build with clocks in
+// the kernel was busy for 2950 of the 3770 cycles of a block pair (32 products of 64.6 cycles, see cdr_attention.cu, are
+// 2067 of them; the rest are barriers, commits and hand-overs).  Measured
 // (B200): 4 x 1024 queries behind 4096 shared keys 167 us, 0.92 PFLOP/s of 1.60 that a large library product reaches; an
-// 8192 prompt with a window of 2048 267 us, 0.90; 8 x 2048 with a window of 512 117 us, 0.52 (masked halves of edge
+// 8192 prompt with a window of 2048 269 us, 0.90; 8 x 2048 with a window of 512 118 us, 0.51 (masked halves of edge
 // blocks, and an epilogue every 5 blocks).
 // Measured and dropped: products cut to the visible keys in every edge block (operand shapes that the issuing warp computes
-// at run time cost it 20 %, 172 -> 205 us on the first case); edge blocks by 32-column chunks that are skipped, masked or
-// plain (2700 cycles per block, unrolled or as a loop, against 2500 for masking the whole score row).
+// at run time: 172 -> 205 us on the first case).
 #include <cuda.h>
 #include <math.h>
 
@@ -44,7 +44,7 @@ namespace {
 
 constexpr int HALF = 128, BQ = 256, BKV = 128;    // rows per half, per tile; keys per block
 constexpr int TA_THREADS = 384, SOFTMAX_WARP0 = 4;
-constexpr int REGS_CONTROL = 88, REGS_SOFTMAX = 208;   // 128*80 + 256*208 <= 384*168, the CTA's allocation at launch
+constexpr int REGS_CONTROL = 88, REGS_SOFTMAX = 208;   // 128*88 + 256*208 <= 384*168, the CTA's allocation at launch
 constexpr int TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;   // + 128 * half
 constexpr float kRescale = 8.0f;                  // log2 units
 constexpr int SINK_COLS = 32;                     // a block of sinks alone is cut to so many keys
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       if constexpr (PACKED) {
         // rows in packed order; 32 columns at a time through shared memory (16-byte pieces of a row XORed with the
         // row), so that four rows of 128 contiguous bytes leave with one instruction: a store per lane of its own
-        // row touches 32 lines and took 10000 cycles per tile
+        // row touches 32 lines
         const int half_rows = a.G * a.Sq * t.seqs_per_half;
         const int64_t at = (static_cast<int64_t>(r.off) * a.Hkv + r.hkv) * t.part_rows + (r.b / t.seqs_per_half + g) * HALF;
         if (row_in_half < half_rows) t.part_lse[at + row_in_half] = none ? -INFINITY : m_ref + __log2f(l);
