@@ -1,6 +1,6 @@
 // Host side of a repeated direct call (conductor_b200/ops.py): checks that the tensors are the ones the call was
 // prepared for, takes the output and the scratch from torch's caching allocator, fills in the pointers and
-// calls the library.  A decode step's kernels take 9 us; the same steps in Python took 9 us on top of the launch.
+// calls the library.  A decode step's kernels take 9 us; host time of the call: 14 us with these steps in Python, 8 us so.
 // Holds no kernel and no pointer of a tensor between calls.
 #include <Python.h>
 
