@@ -1048,7 +1048,9 @@ CachePlan plan_call(const CacheAttn& a) {
       return c;
     }
   }
-  c.path = tile_us < stream_us ? Path::kTile : Path::kStream;
+  // A single query is always streamed: there every row of a task stands at one position, so keys that it does not see are
+  // never multiplied, whatever the cache holds there; a tile would meet them at the edges of its blocks with a weight of 0.
+  c.path = a.Sq > 1 && tile_us < stream_us ? Path::kTile : Path::kStream;
   c.bytes = c.path == Path::kTile ? kTileCounterBytes : stream_bytes(a, c.stream);
   return c;
 }

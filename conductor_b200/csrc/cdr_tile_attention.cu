@@ -705,7 +705,9 @@ int map_prefix(TileArgs& t) {
 
 float tile_attention_us(const CacheAttn& a) {
   const int64_t keys = static_cast<int64_t>(a.window) + (a.Sq < BQ ? a.Sq : BQ);
-  const int64_t blocks = ((keys < a.Skv ? keys : a.Skv) + 2 * BKV - 1) / BKV + (a.P + BKV - 1) / BKV;
+  const int64_t own = (a.Skv + BKV - 1) / BKV, touched = ((keys < a.Skv ? keys : a.Skv) + 2 * BKV - 1) / BKV;
+  const int64_t sinks = ((a.sinks < a.Skv ? a.sinks : a.Skv) + BKV - 1) / BKV;      // in front of the window, as far as there are keys
+  const int64_t blocks = (touched + sinks < own + 1 ? touched + sinks : own + 1) + (a.P + BKV - 1) / BKV;
   const int64_t tiles = static_cast<int64_t>(a.B) * a.Hq * ((a.Sq + BQ - 1) / BQ);
   return 6.0f + (a.D == 128 ? 2.0f : 1.7f) * ((tiles + sm_count() - 1) / sm_count()) * blocks;
 }
