@@ -219,6 +219,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
     sm100::tmem_alloc(tmem_slot, TMEM_COLS);
     sm100::tmem_relinquish();
   }
+  if (PACKED) {
+    // rows of a half above its box: no copy ever writes them, but the product reads them and their lanes have a say in
+    // whether a warp takes a new reference maximum.  Zeros, so that the bits of the others depend on the inputs alone.
+    const int box_rows = a.Sq * a.G * t.seqs_per_half, pieces = (128 - box_rows) * 8;   // 16 bytes each
+    for (int x = threadIdx.x; x < 2 * (HD / 64) * pieces; x += TA_THREADS) {
+      const int part = x / pieces, piece = x - part * pieces;                           // part: 64 columns of a half
+      *reinterpret_cast<uint4*>(smem + L::Q_OFF + part * (128 * 128) + box_rows * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
+    }
+    sm100::fence_proxy_async_smem();
+  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
