@@ -5,7 +5,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -37,6 +38,25 @@ struct CallState {
   cdr_tensor* out_desc = nullptr;
   LaunchMany launch = nullptr;
 };
+
+// What only the dispatcher can serve: modes and tracers that record a call, wrappers of function transforms, and views
+// whose elements are not what the memory holds.
+constexpr c10::DispatchKeySet kDispatched({
+    c10::DispatchKey::Python, c10::DispatchKey::PythonDispatcher, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::PreDispatch,
+    c10::DispatchKey::Tracer, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchDynamicLayerFrontMode,
+    c10::DispatchKey::FuncTorchDynamicLayerBackMode, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched,
+    c10::DispatchKey::FuncTorchBatchedDecomposition, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::BatchedNestedTensor,
+    c10::DispatchKey::VmapMode, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+
+bool calls_are_dispatched() {
+  const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
+  return (tls.included_ - tls.excluded_).has_any(kDispatched);
+}
+
+bool needs_gradient(const at::Tensor& t) {
+  const c10::AutogradState& state = c10::AutogradState::get_tls_state();
+  return (state.get_grad_mode() && t.requires_grad()) || (state.get_fw_grad_mode() && t._fw_grad(0).defined());
+}
 
 struct NoGil {
   PyThreadState* state = PyEval_SaveThread();
@@ -84,19 +104,19 @@ void call_dealloc(PyObject* self) {
   Py_TYPE(self)->tp_free(self);
 }
 
-// run(*tensors): the output; None where the call was made for other tensors (or would need gradients); the library's
-// status where it refused.
+// run(*tensors): the output; None where the call was made for other tensors, would need gradients or is one for the
+// dispatcher; the library's status where it refused.
 PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   CallState& st = *reinterpret_cast<CallObject*>(self)->state;
   if (n != static_cast<Py_ssize_t>(st.ins.size())) Py_RETURN_NONE;
-  const bool grad = c10::GradMode::is_enabled();
+  if (calls_are_dispatched()) Py_RETURN_NONE;
   for (Py_ssize_t i = 0; i < n; ++i) {
     if (!THPVariable_CheckExact(args[i])) Py_RETURN_NONE;
     const at::Tensor& t = THPVariable_Unpack(args[i]);
     const Expected& e = st.ins[i];
     if (t.device() != e.device || t.scalar_type() != e.dtype || t.sizes() != at::IntArrayRef(e.sizes) ||
-        t.strides() != at::IntArrayRef(e.strides) || (grad && t.requires_grad()))
+        t.strides() != at::IntArrayRef(e.strides) || t.key_set().has_any(kDispatched) || needs_gradient(t))
       Py_RETURN_NONE;
     void* p = const_cast<void*>(t.const_data_ptr());
     if (e.aligned && (reinterpret_cast<uintptr_t>(p) & 15u)) Py_RETURN_NONE;
@@ -123,13 +143,26 @@ PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// is_dispatched(*tensors): the call is one for the dispatcher.
+PyObject* is_dispatched(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  bool any = calls_are_dispatched();
+  for (Py_ssize_t i = 0; i < n && !any; ++i) any = THPVariable_Check(args[i]) && THPVariable_Unpack(args[i]).key_set().has_any(kDispatched);
+  return PyBool_FromLong(any);
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef module_methods[] = {
+    {"is_dispatched", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(is_dispatched)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
 PyMethodDef call_methods[] = {
     {"run", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_run)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyTypeObject call_type = {PyVarObject_HEAD_INIT(nullptr, 0) "_cdr_torch.Call", sizeof(CallObject)};
 
-PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_cdr_torch", nullptr, -1, nullptr, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_cdr_torch", nullptr, -1, module_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

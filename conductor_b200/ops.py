@@ -10,7 +10,9 @@ The reference's only attention is ``scaled_dot_product_attention`` over q, k and
 
 Both work on CUDA tensors directly (asynchronously, on the current stream of the tensors' device) and
 in a function compiled with ``backend='gcu'``, where they become one launch of the plan.  They are
-forward-only, like the framework's other attention: a call that would need gradients raises.
+forward-only, like the framework's other attention: a call that would need gradients, backward or forward-mode, raises.
+Calls under a tracer, a dispatch mode or a function transform, and calls with tensor subclasses, go through torch's
+dispatcher as ``torch.ops.conductor.*``.
 
 Common to both: ``q`` is ``[B, Hq, Sq, D]``, the cache ``[B, Hkv, Skv, D]``, ``Hq`` a multiple of ``Hkv``
 (query heads ``h*G .. h*G + G-1`` share key head ``h``); bf16 or f16; ``D`` 64 or 128.  Views are read in
@@ -30,6 +32,8 @@ import threading
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
+from torch.overrides import has_torch_function, has_torch_function_variadic
 
 from .codegen.kernel_templates import CdrLaunchItem, CdrTensor, prefix_attention_launch, window_attention_launch
 from .compiler.executor import attention_view_ok, get_executor, make_descriptors, raise_for_status
@@ -47,18 +51,18 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     ``window >= 1`` counts the query's own position; a window as long as the cache is plain causal
     attention.  ``Sq = 1`` is a decode step over a cache that already holds the new token's key and
     value, ``Sq = Skv`` a prompt, anything between a chunk of a prompt behind a filled cache."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or (q.__class__ is not torch.Tensor and has_torch_function_variadic(q)):
         return torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)
-    return _run_window(q, k, v, window, sinks, lengths, scale)
+    return _run_window(q, k, v, window, sinks, lengths, scale, True)
 
 
 def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                      lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
     """``softmax(scale * q [prefix_k; k]^T) [prefix_v; v]``: every query with ``p >= 0`` sees the whole prefix
     (``[Hkv, P, D]``, ``P >= 0``, the same for all sequences) and the keys ``j <= p`` of its own sequence."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or (q.__class__ is not torch.Tensor and has_torch_function_variadic(q)):
         return torch.ops.conductor.prefix_attention(q, prefix_k, prefix_v, k, v, lengths, scale)
-    return _run_prefix(q, prefix_k, prefix_v, k, v, lengths, scale)
+    return _run_prefix(q, prefix_k, prefix_v, k, v, lengths, scale, True)
 
 
 # ---------------------------------------------------------------- direct calls
@@ -103,7 +107,7 @@ class _Call:
         return out
 
 
-def _run(name, build, params, tensors):
+def _run(name, build, params, tensors, op):
     try:
         call = _calls.last.get((name, params))
     except AttributeError:                         # this thread's first call
@@ -112,22 +116,27 @@ def _run(name, build, params, tensors):
         out = call(tensors)
         if out is not None:
             return out
-    return _other_run(name, build, params, tensors)
+    return _other_run(name, build, params, tensors, op)
 
 
-def _other_run(name, build, params, tensors):
-    """A call that is not the last one of its parameters again: found among the kept ones, or made."""
+def _other_run(name, build, params, tensors, op):
+    """A call that is not the last one of its parameters again: found among the kept ones, or made; with ``op``, left
+    to the dispatcher where something besides the kernel has to see it."""
+    if op is not None and has_torch_function([t for t in tensors if type(t) not in (torch.Tensor, torch.nn.Parameter)]):
+        return op()
     if not all(isinstance(t, torch.Tensor) for t in tensors):
         raise ExecutionError(f"{name}: expected tensors, got {[type(t).__name__ for t in tensors]}", kernel_name=name)
+    if op is not None and any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors):
+        return op()
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")
+    if op is not None and load_call_module().is_dispatched(*tensors):
+        return op()
     for t in tensors:
         if t.device != device:
             raise ExecutionError(f"{name}: tensors on {device} and {t.device}", kernel_name=name)
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
-                                 "torch.no_grad() or detach the inputs", kernel_name=name)
+    _refuse_gradients(name, tensors)
     key = (name, params, *[(t.shape, t.stride(), t.dtype) for t in tensors], device)
     call = _calls.cache.get(key)
     out = call(tensors) if call is not None else None
@@ -146,6 +155,15 @@ def _other_run(name, build, params, tensors):
     return out
 
 
+def _refuse_gradients(name, tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
+                             "torch.no_grad() or detach the inputs", kernel_name=name)
+    if fwAD._current_level >= 0 and fwAD._is_fwd_grad_enabled() and any(fwAD.unpack_dual(t).tangent is not None for t in tensors):
+        raise ExecutionError(f"{name}: an input has a forward-mode gradient but the operator has no such formula; detach "
+                             "the inputs", kernel_name=name)
+
+
 def _build_window(q, window, sinks, has_lengths, scale):
     return window_attention_launch("window_attention", q.shape, q.dtype, window, sinks, has_lengths, scale)
 
@@ -154,18 +172,20 @@ def _build_prefix(q, has_lengths, scale):
     return prefix_attention_launch("prefix_attention", q.shape, q.dtype, has_lengths, scale)
 
 
-def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None):
+def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None, direct=False):
+    op = (lambda: torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)) if direct else None
     window, sinks, scale = operator.index(window), operator.index(sinks), None if scale is None else float(scale)
     if lengths is None:
-        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v))
-    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths))
+        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v), op)
+    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths), op)
 
 
-def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None):
+def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None, direct=False):
+    op = (lambda: torch.ops.conductor.prefix_attention(q, prefix_k, prefix_v, k, v, lengths, scale)) if direct else None
     scale = None if scale is None else float(scale)
     if lengths is None:
-        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v))
-    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths))
+        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v), op)
+    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths), op)
 
 
 # ---------------------------------------------------------------- graph form
@@ -174,6 +194,22 @@ _lib.define("window_attention(Tensor q, Tensor k, Tensor v, int window, int sink
 _lib.define("prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? lengths=None, float? scale=None) -> Tensor")
 _lib.impl("window_attention", _run_window, "CUDA")
 _lib.impl("prefix_attention", _run_prefix, "CUDA")
+
+
+def _no_gradients(name):
+    """The autograd kernel of an operator without a gradient: refuses the call that needs one, else passes it on."""
+    op = getattr(torch.ops.conductor, name).default
+
+    def kernel(*args, **kwargs):
+        _refuse_gradients(name, [t for t in (*args, *kwargs.values()) if isinstance(t, torch.Tensor)])
+        with torch._C._AutoDispatchBelowAutograd():
+            return op(*args, **kwargs)
+
+    return kernel
+
+
+_lib.impl("window_attention", _no_gradients("window_attention"), "Autograd")
+_lib.impl("prefix_attention", _no_gradients("prefix_attention"), "Autograd")
 
 
 @torch.library.register_fake("conductor::window_attention", lib=_lib)

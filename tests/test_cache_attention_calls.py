@@ -1,0 +1,73 @@
+"""Callers and call forms of window_attention and prefix_attention that need no GPU: tracers, transforms, the call module."""
+import ctypes
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+import conductor
+from conductor.compiler.loader import load_call_module
+from conductor.utils.exceptions import ExecutionError
+from conductor_b200.codegen import kernel_templates as kt
+from conductor_b200.csrc.build import build_call_module
+from test_cache_attention import cache
+
+WINDOW, PREFIX = conductor.ops.window_attention, conductor.ops.prefix_attention
+
+
+def test_symbolic_tracing_and_fake_tensors():
+    def both(q, k, v, w, n):
+        return WINDOW(q, k, v, w, 2, lengths=n) + PREFIX(q, k[0], v[0], k, v, lengths=n)
+
+    names = [str(node.target) for node in torch.fx.symbolic_trace(both).graph.nodes if node.op == "call_function"]
+    assert any("window_attention" in n for n in names) and any("prefix_attention" in n for n in names)
+    q, k, v = cache()
+    for device in ("cpu", "cuda"):
+        with FakeTensorMode():
+            args = [torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v)]
+            out = both(*args, 4, torch.zeros(2, dtype=torch.int32, device=device))
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device.type == device
+
+
+def test_the_dispatched_form_refuses_gradients():
+    q, k, v = cache()
+    window, prefix = torch.ops.conductor.window_attention, torch.ops.conductor.prefix_attention
+    for call in (lambda: window(q.clone().requires_grad_(), k, v, 3), lambda: prefix(q, k[0].clone().requires_grad_(), v[0], k, v),
+                 lambda: torch.func.grad(lambda q: window(q, k, v, 3).float().sum())(q),
+                 lambda: torch.func.grad(lambda v: prefix(q, k[0], v[0], k, v=v).float().sum())(v)):
+        with pytest.raises(ExecutionError, match="no backward"):
+            call()
+    with pytest.raises(ExecutionError, match="forward-mode"):
+        torch.func.jvp(lambda q: window(q, k, v, 3), (q,), (torch.ones_like(q),))
+    with fwAD.dual_level(), pytest.raises(ExecutionError, match="forward-mode"):
+        prefix(fwAD.make_dual(q, q), k[0], v[0], k, v)
+
+
+def test_call_module_leaves_to_the_dispatcher_what_is_its(built_library):
+    """Tangents, dispatch modes, tracers and wrapped tensors: the kept call does not take them."""
+    build_call_module()
+    module = load_call_module()
+    item, ins, out = kt.CdrLaunchItem(), (kt.CdrTensor * 3)(), (kt.CdrTensor * 1)()
+    q, k, v = cache()
+    call = module.Call(ctypes.addressof(item), ctypes.addressof(ins), ctypes.addressof(out), 0, (q, k, v))
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    def look(q, k, v):
+        seen.append((call.run(q, k, v), module.is_dispatched(q, k, v)))
+        return q
+
+    assert not module.is_dispatched(q, k, v)
+    with Mode():
+        look(q, k, v)
+    torch.jit.trace(look, (q, k, v), check_trace=False)
+    torch.func.vmap(look)(*(t[None] for t in (q, k, v)))
+    torch.func.functionalize(look)(q, k, v)
+    assert seen == [(None, True)] * 4
+    with fwAD.dual_level():
+        assert call.run(q, fwAD.make_dual(k, k), v) is None

@@ -2,9 +2,11 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from cache_attention_ref import check, reference
-from test_cache_attention_gpu import PREFIX, WINDOW, cache, no_wait_gave_up, rand  # noqa: F401
+from conductor.utils.exceptions import ExecutionError
+from test_cache_attention_gpu import PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,47 @@ def test_hidden_keys_of_a_single_query_with_many_sinks(B, Hq, Hkv, Skv, D, windo
     check(want[few], reference(q[few], k[few], v[few], window=window, sinks=sinks))
     k[:, :, sinks:Skv - window], v[:, :, sinks:Skv - window] = float("nan"), float("inf")
     assert torch.equal(WINDOW(q, k, v, window, sinks), want)
+
+
+def test_forward_mode_is_refused():
+    q, k, v = cache(2, 4, 2, 3, 50, 64)
+    pre = [rand(2, 30, 64, seed=50 + i) for i in range(2)]
+    WINDOW(q, k, v, 20), PREFIX(q, *pre, k, v)                      # the kept form of both calls exists
+    with fwAD.dual_level():
+        d = fwAD.make_dual(q, torch.ones_like(q))
+        for call in (lambda: WINDOW(d, k, v, 20), lambda: torch.ops.conductor.window_attention(d, k, v, 20),
+                     lambda: PREFIX(d, *pre, k, v), lambda: PREFIX(q, fwAD.make_dual(pre[0], pre[1]), pre[1], k, v)):
+            with pytest.raises(ExecutionError, match="forward-mode"):
+                call()
+        WINDOW(q, k, v, 20)                                         # no tangent: as ever
+        with fwAD._set_fwd_grad_enabled(False):
+            WINDOW(d, k, v, 20)
+
+
+def test_function_transforms_are_refused():
+    q, k, v = cache(2, 4, 2, 3, 50, 64)
+    f = lambda q: WINDOW(q, k, v, 20).float().sum()                 # noqa: E731
+    for call in (lambda: torch.func.grad(f)(q), lambda: torch.func.jvp(f, (q,), (torch.ones_like(q),)),
+                 lambda: torch.func.vjp(f, q), lambda: torch.ops.conductor.window_attention(q.clone().requires_grad_(), k, v, 20)):
+        with pytest.raises(ExecutionError, match="backward|forward-mode"):
+            call()
+
+
+def test_tracers_record_the_operators():
+    """What a tracer returns computes the operator on other inputs, not the memory that the traced call filled."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    q, k, v = cache(2, 4, 2, 3, 50, 64)
+    pre = [rand(2, 30, 64, seed=50 + i) for i in range(2)]
+    n = lens(50, 31)
+    both = lambda q, k, v, a, b: WINDOW(q, k, v, 20, 2, lengths=n) + PREFIX(q, a, b, k, v, lengths=n)      # noqa: E731
+    other = [t.flip(0).contiguous() for t in (q, k, v)] + [t.flip(1).contiguous() for t in pre]
+    want = both(*other)
+    g = make_fx(both)(q, k, v, *pre)
+    names = [str(node.target) for node in g.graph.nodes if node.op == "call_function"]
+    assert "conductor.window_attention.default" in names and "conductor.prefix_attention.default" in names
+    assert torch.equal(g(*other), want)
+    traced = torch.jit.trace(both, (q, k, v, *pre))
+    assert "conductor::window_attention" in str(traced.inlined_graph)
+    assert torch.equal(traced(*other), want)
+    assert torch.equal(both(*other), want)
