@@ -3,6 +3,7 @@
 //
 // Replaces the C++ wrapper the reference generates per compiled graph
 // (conductor/compiler/host_wrapper.py:108-197).  No exception leaves this file.
+#include <cuda.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -66,6 +67,22 @@ int sm_count() {
     g_sm_count[dev] = n;  // benign race: every writer stores the same value
   }
   return g_sm_count[dev];
+}
+
+// A host thread that has made no CUDA call yet has no context bound to it.  The runtime binds one in its own calls, but
+// tensor maps and run-time instances go to the driver, which refuses such a thread (error 201), and everything in front of
+// them may be cached.  A context that the thread has, the caller's own included, stays as it is.
+static void bind_context() {
+  typedef CUresult (*CtxGetCurrent)(CUcontext*);
+  static const CtxGetCurrent get = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<CtxGetCurrent>(p);
+  }();
+  CUcontext ctx = nullptr;
+  int dev = 0;
+  if (get && (get(&ctx) != CUDA_SUCCESS || !ctx) && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
 }
 
 void clear_error() { g_error[0] = 0; }
@@ -253,6 +270,7 @@ int cdr_launch(int template_id, const cdr_tensor* inputs, int n_inputs, const cd
   g_error[0] = 0;
   if (int rc = check_lists(inputs, n_inputs, outputs, n_outputs)) return rc;
   if (int rc = check_params(template_id, params, params_bytes)) return rc;
+  bind_context();
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   switch (template_id) {
     case CDR_T_ELEMENTWISE:

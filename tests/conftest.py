@@ -20,6 +20,8 @@ GOLDEN = Path(__file__).resolve().parent / "golden"
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: test needs a CUDA device")
+    # a test whose worker thread died has not seen what it was there to see
+    config.addinivalue_line("filterwarnings", "error::pytest.PytestUnhandledThreadExceptionWarning")
 
 
 def pytest_collection_modifyitems(config, items):

@@ -1,4 +1,5 @@
 """How window_attention and prefix_attention may be called: threads, transforms and tracers, views, single queries, repeats."""
+import threading
 
 import pytest
 import torch
@@ -6,9 +7,54 @@ import torch.autograd.forward_ad as fwAD
 
 from cache_attention_ref import check, reference
 from conductor.utils.exceptions import ExecutionError
+from conductor_b200.compiler.gcu_backend import get_gcu_backend
 from test_cache_attention_gpu import PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+
+def in_a_new_thread(fn):
+    """fn's result from a host thread that has made no CUDA call before; what it raises is raised here."""
+    box = []
+
+    def work():
+        try:
+            box.append((fn(), None))
+        except BaseException as exc:  # noqa: BLE001 -- handed to the caller
+            box.append((None, exc))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    out, exc = box[0]
+    if exc is not None:
+        raise exc
+    return out
+
+
+def test_calls_from_a_thread_without_a_context():
+    """A new host thread has no CUDA context bound to it; everything it needs may be cached by then, so that no
+    runtime call binds one before the library asks the driver for a tensor map or launches a run-time instance."""
+    q, k, v = cache(4, 8, 2, 1, 600, 128)
+    qp, kp, vp = cache(2, 4, 4, 300, 300, 128)
+    pre = [rand(2, 3000, 128, seed=50 + i) for i in range(2)]
+    x, w, b = rand(300, 256), rand(512, 256, seed=1), rand(512, seed=2)
+    torch._dynamo.reset()
+    get_gcu_backend().clear_cache()
+    plans = []
+    for fn, args in ((lambda x, w, b: torch.relu(torch.nn.functional.linear(x, w, b)), (x, w, b)),
+                     (lambda q, k, v: torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True), (qp, kp, vp)),
+                     (lambda x: torch.relu(x * 1.25 - 0.5) * torch.sigmoid(x) + 3.0 * x, (x,))):      # a run-time instance
+        torch.compile(fn, backend="gcu")(*args)
+        plans.append((list(get_gcu_backend()._compiled_functions.values())[-1], args))
+    calls = [lambda: WINDOW(q, k, v, 256, 4), lambda: WINDOW(qp, kp, vp, 100, 4), lambda: PREFIX(q, *pre, k, v)]
+    calls += [lambda p=p, a=a: p(*a)[0] for p, a in plans]
+    for call in calls:
+        want = call().clone()
+        call()                                   # leaves a free block of every size the call takes
+        torch.cuda.synchronize()
+        for _ in range(2):
+            assert torch.equal(in_a_new_thread(call), want)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
