@@ -891,6 +891,8 @@ int check_operand(const cdr_tensor& t, const char* op, const char* name, int ran
   if (t.rank != rank) { set_error("%s: %s has rank %d, expected %d", op, name, t.rank, rank); return CDR_ERR_BAD_ARG; }
   if (t.dtype != dtype) { set_error("%s: %s differs from q in dtype", op, name); return CDR_ERR_BAD_ARG; }
   if (t.shape[rank - 1] != D) { set_error("%s: %s has head dimension %lld, q has %lld", op, name, (long long)t.shape[rank - 1], (long long)D); return CDR_ERR_BAD_ARG; }
+  *st = HeadStrides{D, D, D};
+  if (numel(t) == 0) return CDR_OK;      // never addressed: whatever strides a view of nothing has
   if (t.stride[rank - 1] != 1) { set_error("%s: the head dimension of %s must be contiguous", op, name); return CDR_ERR_UNSUPPORTED; }
   int64_t s[3] = {D, D, D};
   for (int i = 0; i < rank - 1; ++i) {

@@ -12,7 +12,8 @@ from conductor.compiler.loader import load_call_module
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.codegen import kernel_templates as kt
 from conductor_b200.csrc.build import build_call_module
-from test_cache_attention import cache
+from conductor_b200.codegen.operator_registry import Template
+from test_cache_attention import _workspace, cache
 
 WINDOW, PREFIX = conductor.ops.window_attention, conductor.ops.prefix_attention
 
@@ -71,3 +72,10 @@ def test_call_module_leaves_to_the_dispatcher_what_is_its(built_library):
     assert seen == [(None, True)] * 4
     with fwAD.dual_level():
         assert call.run(q, fwAD.make_dual(k, k), v) is None
+
+
+def test_strides_of_empty_operands_do_not_matter(built_library):
+    q = cache()[0]
+    for t in (torch.zeros(2, 2, 9, 67, dtype=q.dtype)[..., :64][:, :, :0], torch.zeros(2, 2, 64, 9, dtype=q.dtype).transpose(2, 3)[:, :, :0]):
+        assert _workspace(Template.WINDOW_ATTENTION, [q, t, t], torch.empty_like(q), kt.CdrWindowAttnParams(0.1, 0, 4, 0))[0] == 0
+        assert _workspace(Template.PREFIX_ATTENTION, [q, t[0], t[0], t, t], torch.empty_like(q), kt.CdrPrefixAttnParams(0.1, 0))[0] == 0

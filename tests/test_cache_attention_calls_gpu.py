@@ -127,3 +127,14 @@ def test_tracers_record_the_operators():
     assert "conductor::window_attention" in str(traced.inlined_graph)
     assert torch.equal(traced(*other), want)
     assert torch.equal(both(*other), want)
+
+
+def test_views_of_empty_tensors():
+    """An empty cache or prefix has no element to read: its strides do not matter."""
+    q = rand(2, 4, 3, 64)
+    odd = rand(2, 2, 9, 67)[..., :64][:, :, :0]
+    turned = rand(2, 2, 64, 9).transpose(2, 3)[:, :, :0]
+    for t in (odd, turned):
+        assert torch.equal(WINDOW(q, t, t, 5), torch.zeros_like(q))
+        k, v = rand(2, 2, 50, 64, seed=1), rand(2, 2, 50, 64, seed=2)
+        assert torch.equal(PREFIX(q, t[0], t[0], k, v), WINDOW(q, k, v, 1 << 20))
