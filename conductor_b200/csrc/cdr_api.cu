@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <mutex>
@@ -83,6 +84,11 @@ static void bind_context() {
   CUcontext ctx = nullptr;
   int dev = 0;
   if (get && (get(&ctx) != CUDA_SUCCESS || !ctx) && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
+
+bool pdl_enabled() {
+  static const bool on = getenv("CDR_DISABLE_PDL") == nullptr;
+  return on;
 }
 
 void clear_error() { g_error[0] = 0; }

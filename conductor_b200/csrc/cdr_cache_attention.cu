@@ -819,7 +819,7 @@ int launch_stream_cfg(const StreamArgs& s, const StreamPlan& p, int tpr, cudaStr
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.blockDim = dim3(L::THREADS, 1, 1);

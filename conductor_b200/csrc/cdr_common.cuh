@@ -60,6 +60,9 @@ int sm_count();
 // Device pointer of the current device's status word (0 = ok; set by a kernel whose bounded
 // wait gave up).  nullptr if it cannot be obtained; kernels accept that.
 int* device_status_ptr();
+// Launches may start before the kernel in front of them has ended (programmatic dependent launch); CDR_DISABLE_PDL in the
+// environment of the process's first launch puts them one after the other, to isolate an ordering problem.
+bool pdl_enabled();
 
 // Per-template launchers (defined in the template's .cu file).
 int launch_elementwise(const cdr_tensor* ins, int n_in, const cdr_tensor* outs, int n_out,

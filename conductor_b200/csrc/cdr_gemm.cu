@@ -673,7 +673,6 @@ int launch_gemm_epilogue(const cdr_tensor* ins, int n_in, const cdr_tensor* outs
     configured = true;
   }
 
-  static const bool pdl = getenv("CDR_DISABLE_PDL") == nullptr;
   // Few large tiles leave most SMs idle: when the 256 x 256 pair tiles fill less than half of the
   // CTA pairs and 128 x 128 tiles would still fit in one wave, run the 1-CTA kernel on 128 x 128
   // tiles instead (a 1024 x 1024 x 4096 product: 16 pair tiles on 74 pairs, or 64 tiles on 148 SMs).
@@ -701,7 +700,7 @@ int launch_gemm_epilogue(const cdr_tensor* ins, int n_in, const cdr_tensor* outs
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     if (dt == CDR_BF16) CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_epilogue_pair_kernel<true>, a));
@@ -724,7 +723,7 @@ int launch_gemm_epilogue(const cdr_tensor* ins, int n_in, const cdr_tensor* outs
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (narrow) {

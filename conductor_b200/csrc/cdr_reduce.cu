@@ -375,11 +375,6 @@ RowChain match_row_chain(const cdr_ew_params& p, int dt, int* full_idx, int* row
   return kRNone;
 }
 
-inline bool pdl_enabled() {
-  static const bool on = getenv("CDR_DISABLE_PDL") == nullptr;
-  return on;
-}
-
 template <class Chain, int NT, int VPT, int RB, bool EXACT>
 int launch_named_variant(const RowArgs& a, cudaStream_t s) {
   auto kern = row_reduce_named_kernel<Chain, NT, VPT, RB, EXACT>;

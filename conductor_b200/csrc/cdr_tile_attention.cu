@@ -681,7 +681,7 @@ int launch_tile_cfg(TileArgs& t, int64_t tiles, int ctas, void* counter, cudaStr
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   CDR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, t));

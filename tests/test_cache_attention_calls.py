@@ -11,7 +11,7 @@ import conductor
 from conductor.compiler.loader import load_call_module
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.codegen import kernel_templates as kt
-from conductor_b200.csrc.build import build_call_module
+from conductor_b200.csrc.build import CSRC, build_call_module
 from conductor_b200.codegen.operator_registry import Template
 from test_cache_attention import _workspace, cache
 
@@ -79,3 +79,12 @@ def test_strides_of_empty_operands_do_not_matter(built_library):
     for t in (torch.zeros(2, 2, 9, 67, dtype=q.dtype)[..., :64][:, :, :0], torch.zeros(2, 2, 64, 9, dtype=q.dtype).transpose(2, 3)[:, :, :0]):
         assert _workspace(Template.WINDOW_ATTENTION, [q, t, t], torch.empty_like(q), kt.CdrWindowAttnParams(0.1, 0, 4, 0))[0] == 0
         assert _workspace(Template.PREFIX_ATTENTION, [q, t[0], t[0], t, t], torch.empty_like(q), kt.CdrPrefixAttnParams(0.1, 0))[0] == 0
+
+
+def test_every_launch_obeys_the_switch_that_puts_kernels_one_after_the_other():
+    sources = [(f.name, line) for f in sorted(CSRC.glob("*.cu*")) for line in f.read_text().splitlines()]
+    allowed = [(name, line) for name, line in sources if "programmaticStreamSerializationAllowed" in line]
+    assert {name for name, _ in allowed} >= {"cdr_cache_attention.cu", "cdr_tile_attention.cu", "cdr_gemm.cu", "cdr_reduce.cu"}
+    for name, line in allowed:
+        assert "pdl_enabled()" in line, (name, line)
+    assert sum("CDR_DISABLE_PDL" in line and "getenv" in line for _, line in sources) == 1

@@ -1,5 +1,9 @@
 """How window_attention and prefix_attention may be called: threads, transforms and tracers, views, single queries, repeats."""
+import os
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -11,6 +15,7 @@ from conductor_b200.compiler.gcu_backend import get_gcu_backend
 from test_cache_attention_gpu import PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
 
 
 def in_a_new_thread(fn):
@@ -138,3 +143,28 @@ def test_views_of_empty_tensors():
         assert torch.equal(WINDOW(q, t, t, 5), torch.zeros_like(q))
         k, v = rand(2, 2, 50, 64, seed=1), rand(2, 2, 50, 64, seed=2)
         assert torch.equal(PREFIX(q, t[0], t[0], k, v), WINDOW(q, k, v, 1 << 20))
+
+
+def test_the_same_bits_with_kernels_one_after_the_other(tmp_path):
+    """CDR_DISABLE_PDL=1: no kernel starts before the one in front of it has ended; the results are the same."""
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from test_cache_attention_gpu import PREFIX, WINDOW, cache, lens, rand
+q, k, v = cache(20, 8, 2, 1, 600, 128)
+n = torch.arange(20, device="cuda", dtype=torch.int32) * 30
+pre = [rand(2, 3000, 128, seed=50 + i) for i in range(2)]
+few = [t[:2].contiguous() for t in (q, k, v)]
+long = cache(20, 8, 2, 300, 300, 64)
+out = []
+for _ in range(3):
+    out += [WINDOW(q, k, v, 256, 4, lengths=n), PREFIX(q, *pre, k, v, lengths=n), WINDOW(*few, 100), PREFIX(*few[:1], *pre, *few[1:]), WINDOW(*long, 100, 4)]
+torch.save([t.cpu() for t in out], sys.argv[1])
+""" % (str(ROOT), str(ROOT / "tests"))
+    got = []
+    for i, extra in enumerate(({}, {"CDR_DISABLE_PDL": "1"})):
+        path = tmp_path / f"{i}.pt"
+        subprocess.run([sys.executable, "-c", code, str(path)], env={**os.environ, **extra}, check=True, timeout=300)
+        got.append(torch.load(path))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
