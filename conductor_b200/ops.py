@@ -20,7 +20,7 @@ place when ``D`` is contiguous and the other strides are multiples of 8 elements
 gathered first.  ``lengths`` (``[B]``, int32 or int64, on the same device) is how many keys each
 sequence uses, clamped to ``0 .. Skv``; what the cache holds behind them does not matter.  Query ``i`` stands
 at position ``p = L - Sq + i``; a query with ``p < 0`` sees nothing, and a query that sees nothing
-returns 0.  ``scale`` defaults to ``1 / sqrt(D)`` and is positive.  The result is contiguous ``[B, Hq, Sq, D]``.
+returns 0.  ``scale`` defaults to ``1 / sqrt(D)`` and is positive (a constant inside compiled functions).  The result is contiguous ``[B, Hq, Sq, D]``.
 Among the keys in use, a non-finite value of ``k`` or ``v`` that some queries see and others do not may reach the others too
 (0 times infinity); with ``Sq = 1`` hidden keys may hold anything.
 """
@@ -51,7 +51,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     ``window >= 1`` counts the query's own position; a window as long as the cache is plain causal
     attention.  ``Sq = 1`` is a decode step over a cache that already holds the new token's key and
     value, ``Sq = Skv`` a prompt, anything between a chunk of a prompt behind a filled cache."""
-    if torch.compiler.is_compiling() or (q.__class__ is not torch.Tensor and has_torch_function_variadic(q)):
+    if torch.compiler.is_compiling():
+        # plans hold both as constants: an argument that changes from call to call makes another plan
+        window, sinks = operator.index(window), operator.index(sinks)
+        return torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)
+    if q.__class__ is not torch.Tensor and has_torch_function_variadic(q):
         return torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)
     return _run_window(q, k, v, window, sinks, lengths, scale, True)
 

@@ -8,6 +8,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import conductor
+from conductor.compiler.jit_compiler import ChoreoJITCompiler
 from conductor.compiler.loader import load_call_module
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.codegen import kernel_templates as kt
@@ -88,3 +89,20 @@ def test_every_launch_obeys_the_switch_that_puts_kernels_one_after_the_other():
     for name, line in allowed:
         assert "pdl_enabled()" in line, (name, line)
     assert sum("CDR_DISABLE_PDL" in line and "getenv" in line for _, line in sources) == 1
+
+
+def test_window_and_sinks_may_change_from_call_to_call_of_a_compiled_function():
+    torch._dynamo.reset()
+    q, k, v = cache()
+    seen = []
+
+    def backend(gm, example):
+        p = ChoreoJITCompiler().compile_graph(gm, example).launches[-1].params
+        seen.append((p.window, p.sinks))
+        return lambda *a: (torch.empty_like(q),)
+
+    f = torch.compile(lambda q, k, v, w, s: conductor.ops.window_attention(q, k, v, w, s), backend=backend)
+    numbers = [(5, 1), (6, 2), (7, 0), (70, 30)]
+    for w, s in numbers:
+        f(q, k, v, w, s)
+    assert seen == numbers

@@ -9,6 +9,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
+import conductor
 from cache_attention_ref import check, reference
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.compiler.gcu_backend import get_gcu_backend
@@ -143,6 +144,33 @@ def test_views_of_empty_tensors():
         assert torch.equal(WINDOW(q, t, t, 5), torch.zeros_like(q))
         k, v = rand(2, 2, 50, 64, seed=1), rand(2, 2, 50, 64, seed=2)
         assert torch.equal(PREFIX(q, t[0], t[0], k, v), WINDOW(q, k, v, 1 << 20))
+
+
+def test_views_inside_and_into_compiled_functions():
+    """Token-major caches, slices and a fused projection: as graph inputs (read in place) and made in the graph (gathered)."""
+    B, Hq, Hkv, Sq, Skv, D = 3, 8, 2, 5, 120, 64
+    q, k, v = cache(B, Hq, Hkv, Sq, Skv, D)
+    n = lens(120, 77, 4)
+    want = reference(q, k, v, window=40, sinks=3, lengths=n)
+    turned = [t.transpose(1, 2).contiguous() for t in (q, k, v)]
+    torch._dynamo.reset()
+    outside = torch.compile(lambda q, k, v, n: conductor.ops.window_attention(q, k, v, 40, 3, lengths=n), backend="gcu")
+    check(outside(*(t.transpose(1, 2) for t in turned), n), want, "views as inputs")
+    inside = torch.compile(lambda q, k, v, n: conductor.ops.window_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), 40, 3, lengths=n),
+                           backend="gcu")
+    check(inside(*turned, n), want, "views in the graph")
+    longer = [torch.cat([t, t.flip(2)], 2) for t in (k, v)]
+    sliced = torch.compile(lambda q, k, v, n: conductor.ops.window_attention(q, k[:, :, :Skv], v[:, :, :Skv], 40, 3, lengths=n), backend="gcu")
+    check(sliced(q, *longer, n), want, "slices in the graph")
+
+
+def test_numbers_of_a_compiled_function_change():
+    """Window and sinks are plain numbers of the call: other values are another plan, not a refusal."""
+    q, k, v = cache(2, 4, 2, 3, 90, 64)
+    torch._dynamo.reset()
+    f = torch.compile(lambda q, k, v, w, s: conductor.ops.window_attention(q, k, v, w, s), backend="gcu")
+    for w, s in ((5, 1), (6, 2), (70, 30), (7, 3)):
+        check(f(q, k, v, w, s), reference(q, k, v, window=w, sinks=s), f"{w} {s}")
 
 
 def test_the_same_bits_with_kernels_one_after_the_other(tmp_path):
