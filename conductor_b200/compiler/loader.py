@@ -19,6 +19,7 @@ LIB_NAME = "libconductor_b200.so"
 ABI_VERSION = 1
 
 _lib: Optional[ctypes.CDLL] = None
+_call_module = None
 
 # name -> (restype, argtypes): every symbol include/conductor_b200.h declares
 _c = ctypes
@@ -80,12 +81,21 @@ def load_library(build_if_missing: bool = False) -> ctypes.CDLL:
 
 
 def load_call_module():
-    """The compiled host side of direct operator calls (``csrc/cdr_torch.cpp``)."""
+    """The compiled host side of direct operator calls (``csrc/cdr_torch.cpp``), built for this torch and this Python."""
+    global _call_module
+    if _call_module is not None:
+        return _call_module
+    from ..csrc.build import call_module_identity
+
     try:
         from ..csrc import _cdr_torch
     except ImportError as exc:
         raise DeviceError("the call module of conductor_b200.ops is missing or does not fit this torch "
                           f"({exc}); run `python -m conductor_b200.csrc.build`") from exc
+    if _cdr_torch.built_for != call_module_identity():
+        raise DeviceError(f"the call module of conductor_b200.ops was built for {_cdr_torch.built_for}, this is "
+                          f"{call_module_identity()}; run `python -m conductor_b200.csrc.build`")
+    _call_module = _cdr_torch
     return _cdr_torch
 
 

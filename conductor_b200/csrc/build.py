@@ -12,6 +12,8 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -20,6 +22,7 @@ LIB_NAME = "libconductor_b200.so"
 LIB_PATH = CSRC / LIB_NAME
 CALL_MODULE_SOURCE = "cdr_torch.cpp"               # CPython module, linked against torch (conductor_b200/ops.py)
 CALL_MODULE_PATH = CSRC / "_cdr_torch.so"
+CALL_MODULE_STAMP = CSRC / "_cdr_torch.stamp"      # what the module was built for
 
 # file -> extra flags.  The elementwise and reduction templates must not contract
 # a*b+c into an fma: eager rounds the product and the sum separately.
@@ -69,35 +72,48 @@ def _compile(src: str, flags: list[str], verbose: bool) -> Path:
     return obj
 
 
-def build_call_module(force: bool = False) -> Path:
-    """Compile the host side of direct calls against the installed torch; returns its path."""
-    import sysconfig
-
+def call_module_identity() -> str:
+    """The torch and the Python whose class layouts the call module is compiled against."""
     import torch
 
-    src = CSRC / CALL_MODULE_SOURCE
+    return f"torch {torch.__version__} {sysconfig.get_config_var('SOABI')}"
+
+
+def build_call_module(force: bool = False) -> Path:
+    """Compile the host side of direct calls against the installed torch; returns its path."""
+    import torch
+
+    src, identity = CSRC / CALL_MODULE_SOURCE, call_module_identity()
     newest = max(src.stat().st_mtime, (CSRC.parent.parent / "include" / "conductor_b200.h").stat().st_mtime)
-    if not force and CALL_MODULE_PATH.exists() and CALL_MODULE_PATH.stat().st_mtime >= newest:
+    fits = CALL_MODULE_STAMP.exists() and CALL_MODULE_STAMP.read_text() == identity
+    if not force and fits and CALL_MODULE_PATH.exists() and CALL_MODULE_PATH.stat().st_mtime >= newest:
         return CALL_MODULE_PATH
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DCDR_BUILT_FOR="{identity}"',
            f"-isystem{root}/include", f"-isystem{root}/include/torch/csrc/api/include",
            f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda}/include",
            str(src), "-o", str(CALL_MODULE_PATH), f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    CALL_MODULE_STAMP.write_text(identity)
     return CALL_MODULE_PATH
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every kernel template, link the shared library and build the call module; returns the library's path."""
+    """Compile every kernel template, link the shared library and build the call module; returns the library's path.
+
+    Without a C++ compiler or torch's headers the library stands alone: callers of the C ABI and compiled graphs need
+    nothing else, and a direct operator call says what it misses."""
     with ThreadPoolExecutor(max_workers=1) as side:
         module = side.submit(build_call_module, force)
         path = build_library(force, verbose)
-        module.result()
+        try:
+            module.result()
+        except Exception as exc:
+            warnings.warn(f"the call module of conductor_b200.ops was not built: {exc}", RuntimeWarning, stacklevel=2)
     return path
 
 

@@ -174,6 +174,10 @@ PyMODINIT_FUNC PyInit__cdr_torch(void) {
   if (PyType_Ready(&call_type) < 0) return nullptr;
   PyObject* m = PyModule_Create(&module_def);
   if (!m) return nullptr;
+  if (PyModule_AddStringConstant(m, "built_for", CDR_BUILT_FOR) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
   Py_INCREF(&call_type);
   if (PyModule_AddObject(m, "Call", reinterpret_cast<PyObject*>(&call_type)) < 0) {
     Py_DECREF(&call_type);

@@ -1,5 +1,6 @@
 """Callers and call forms of window_attention and prefix_attention that need no GPU: tracers, transforms, the call module."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -8,10 +9,12 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import conductor
+from conductor.compiler import loader
 from conductor.compiler.jit_compiler import ChoreoJITCompiler
 from conductor.compiler.loader import load_call_module
-from conductor.utils.exceptions import ExecutionError
+from conductor.utils.exceptions import DeviceError, ExecutionError
 from conductor_b200.codegen import kernel_templates as kt
+from conductor_b200.csrc import build
 from conductor_b200.csrc.build import CSRC, build_call_module
 from conductor_b200.codegen.operator_registry import Template
 from test_cache_attention import _workspace, cache
@@ -106,3 +109,37 @@ def test_window_and_sinks_may_change_from_call_to_call_of_a_compiled_function():
     for w, s in numbers:
         f(q, k, v, w, s)
     assert seen == numbers
+
+
+def test_call_module_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    """A module of another torch or Python is built again however new its file is, and is not loaded."""
+    ran = []
+    monkeypatch.setattr(build, "CALL_MODULE_PATH", tmp_path / "_cdr_torch.so")
+    monkeypatch.setattr(build, "CALL_MODULE_STAMP", tmp_path / "_cdr_torch.stamp")
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: ran.append(cmd) or types.SimpleNamespace(returncode=0, stdout="", stderr=""))
+    build.CALL_MODULE_PATH.write_bytes(b"")
+    build.CALL_MODULE_STAMP.write_text("torch 1.0 cpython-30")
+    build.build_call_module()
+    assert len(ran) == 1 and build.CALL_MODULE_STAMP.read_text() == build.call_module_identity()
+    build.build_call_module()
+    assert len(ran) == 1
+
+
+def test_call_module_of_another_torch_is_not_loaded(built_library, monkeypatch):
+    build_call_module()
+    monkeypatch.setattr(loader, "_call_module", None)
+    assert loader.load_call_module().built_for == build.call_module_identity()
+    monkeypatch.setattr(loader, "_call_module", None)
+    monkeypatch.setattr(build, "call_module_identity", lambda: "torch 1.0 cpython-30")
+    with pytest.raises(DeviceError, match="was built for"):
+        loader.load_call_module()
+
+
+def test_the_library_is_built_without_the_call_module(monkeypatch):
+    def fails(force=False):
+        raise FileNotFoundError("g++")
+
+    monkeypatch.setattr(build, "build_call_module", fails)
+    monkeypatch.setattr(build, "build_library", lambda force=False, verbose=False: build.LIB_PATH)
+    with pytest.warns(RuntimeWarning, match="call module"):
+        assert build.build() == build.LIB_PATH
