@@ -98,7 +98,7 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   return r;
 }
 
-// The keys a task reads, as up to three ranges of units of 16: prefix, sinks, window.
+// The keys a task reads, as up to three ranges of units of 32 (SA_KEYS): prefix, sinks, window.
 struct KeyRanges {
   int prefix_end, sink_end, lo, hi;
   int n_prefix, n_sink, n_total;   // units, cumulated

@@ -64,7 +64,7 @@ struct StreamPlan {
   int64_t tasks, slots, units;     // units of 32 keys: the most there can be (every sequence at full length)
 };
 
-// Many query rows (cdr_tile_attention.cu).  `ws` starts with kTileCounterBytes for the tile counter, 32-byte aligned.
+// Many query rows (cdr_tile_attention.cu).  Their `ws` is kTileCounterBytes for the tile counter, 32-byte aligned.
 constexpr size_t kTileCounterBytes = 256;
 // prefix, sinks and window of every (sequence, query head), 256 queries per tile
 int launch_tile_attention(const CacheAttn& a, void* ws, cudaStream_t stream);
@@ -72,7 +72,7 @@ float tile_attention_us(const CacheAttn& a);   // estimated time
 // the shared prefix alone, for G * Sq <= 128 query rows per sequence and key head, into *part in `ws`; `own_units`: of the
 // streaming kernel that runs beside it
 PackedPlan plan_packed(const CacheAttn& a, int64_t own_units);
-size_t packed_workspace(const CacheAttn& a, const PackedPlan& plan);   // with the counter
+size_t packed_workspace(const CacheAttn& a, const PackedPlan& plan);
 int launch_packed_prefix(const CacheAttn& a, const PackedPlan& plan, void* ws, PrefixPartials* part, cudaStream_t stream);
 
 #ifdef __CUDACC__

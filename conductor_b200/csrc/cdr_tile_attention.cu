@@ -779,7 +779,7 @@ PackedPlan plan_packed(const CacheAttn& a, int64_t own_units) {
 }
 
 size_t packed_workspace(const CacheAttn& a, const PackedPlan& p) {
-  return kTileCounterBytes + static_cast<size_t>(p.splits) * a.Hkv * p.row_tiles * 2 * HALF * (a.D + 1) * sizeof(float);
+  return static_cast<size_t>(p.splits) * a.Hkv * p.row_tiles * 2 * HALF * (a.D + 1) * sizeof(float);
 }
 
 int launch_packed_prefix(const CacheAttn& a, const PackedPlan& plan, void* ws, PrefixPartials* part, cudaStream_t stream) {
@@ -792,12 +792,12 @@ int launch_packed_prefix(const CacheAttn& a, const PackedPlan& plan, void* ws, P
   const int64_t rows = static_cast<int64_t>(plan.row_tiles) * 2 * HALF;
   if (rows > 0x3fffffff) { set_error("attention: too many sequences"); return CDR_ERR_UNSUPPORTED; }
   t.part_rows = static_cast<int>(rows);
-  t.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kTileCounterBytes);
+  t.part_o = static_cast<float*>(ws);
   t.part_lse = t.part_o + static_cast<size_t>(t.splits) * a.Hkv * rows * a.D;
   if (int rc = map_heads(&t.tmap_q, a.q, a, a.Sq, a.Hq, a.B, a.sq, 64, a.Sq, a.G, t.seqs_per_half, 128)) return rc;
   if (int rc = map_prefix(t)) return rc;
   *part = PrefixPartials{t.part_o, t.part_lse, t.splits, t.part_rows, t.seqs_per_half};
-  return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, plan.ctas, ws, stream);
+  return launch_tile_typed<true>(t, static_cast<int64_t>(t.splits) * a.Hkv * t.n_qtiles, plan.ctas, nullptr, stream);
 }
 
 }  // namespace cdr

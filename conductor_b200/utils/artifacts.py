@@ -24,7 +24,8 @@ from .logging import get_logger
 logger = get_logger(__name__)
 
 _TEMPLATE_NAMES = {0: "alias", 1: "elementwise", 2: "row_reduce", 3: "softmax_fwd", 4: "softmax_bwd",
-                   5: "gemm_epilogue", 6: "attention", 7: "full_reduce", 8: "layer_norm"}
+                   5: "gemm_epilogue", 6: "attention", 7: "full_reduce", 8: "layer_norm", 9: "copy", 10: "col_sum",
+                   11: "window_attention", 12: "prefix_attention"}
 _KINDS = ("fx", "dag", "clusters", "plan", "source")
 
 

@@ -1,5 +1,6 @@
 """Callers and call forms of window_attention and prefix_attention that need no GPU: tracers, transforms, the call module."""
 import ctypes
+import json
 import types
 
 import pytest
@@ -17,7 +18,8 @@ from conductor_b200.codegen import kernel_templates as kt
 from conductor_b200.csrc import build
 from conductor_b200.csrc.build import CSRC, build_call_module
 from conductor_b200.codegen.operator_registry import Template
-from test_cache_attention import _workspace, cache
+from conductor_b200.utils.artifacts import DebugArtifactManager
+from test_cache_attention import _workspace, cache, compile_plan
 
 WINDOW, PREFIX = conductor.ops.window_attention, conductor.ops.prefix_attention
 
@@ -143,3 +145,18 @@ def test_the_library_is_built_without_the_call_module(monkeypatch):
     monkeypatch.setattr(build, "build_library", lambda force=False, verbose=False: build.LIB_PATH)
     with pytest.warns(RuntimeWarning, match="call module"):
         assert build.build() == build.LIB_PATH
+
+
+def test_a_compiled_call_with_a_window_of_nothing_is_refused():
+    q, k, v = cache()
+    for window, sinks in ((0, 0), (3, -1)):
+        with pytest.raises(Exception, match="window must be at least 1 and sinks at least 0"):
+            compile_plan(lambda q, k, v: conductor.ops.window_attention(q, k, v, window, sinks), q, k, v)
+
+
+def test_debug_artifacts_name_the_operators(tmp_path):
+    q, k, v = cache()
+    plan = compile_plan(lambda q, k, v: conductor.ops.prefix_attention(conductor.ops.window_attention(q, k, v, 5), k[0], v[0], k, v), q, k, v)
+    path = DebugArtifactManager(str(tmp_path)).save_clusters("kernel", plan.launches)
+    names = [row["template"] for row in json.loads(path.read_text())]
+    assert "window_attention" in names and "prefix_attention" in names and not any(n.isdigit() for n in names)
