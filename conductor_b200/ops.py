@@ -111,7 +111,7 @@ class _Call:
         return out
 
 
-def _run(name, build, params, tensors, op):
+def _run(name, build, params, tensors, direct):
     try:
         call = _calls.last.get((name, params))
     except AttributeError:                         # this thread's first call
@@ -120,23 +120,23 @@ def _run(name, build, params, tensors, op):
         out = call(tensors)
         if out is not None:
             return out
-    return _other_run(name, build, params, tensors, op)
+    return _other_run(name, build, params, tensors, direct)
 
 
-def _other_run(name, build, params, tensors, op):
-    """A call that is not the last one of its parameters again: found among the kept ones, or made; with ``op``, left
+def _other_run(name, build, params, tensors, direct):
+    """A call that is not the last one of its parameters again: found among the kept ones, or made; a direct call is left
     to the dispatcher where something besides the kernel has to see it."""
-    if op is not None and has_torch_function([t for t in tensors if type(t) not in (torch.Tensor, torch.nn.Parameter)]):
-        return op()
+    if direct and has_torch_function([t for t in tensors if type(t) not in (torch.Tensor, torch.nn.Parameter)]):
+        return _dispatched(name, params, tensors)
     if not all(isinstance(t, torch.Tensor) for t in tensors):
         raise ExecutionError(f"{name}: expected tensors, got {[type(t).__name__ for t in tensors]}", kernel_name=name)
-    if op is not None and any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors):
-        return op()
+    if direct and any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors):
+        return _dispatched(name, params, tensors)
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")
-    if op is not None and load_call_module().is_dispatched(*tensors):
-        return op()
+    if direct and load_call_module().is_dispatched(*tensors):
+        return _dispatched(name, params, tensors)
     for t in tensors:
         if t.device != device:
             raise ExecutionError(f"{name}: tensors on {device} and {t.device}", kernel_name=name)
@@ -159,6 +159,12 @@ def _other_run(name, build, params, tensors, op):
     return out
 
 
+def _dispatched(name, params, tensors):
+    *numbers, has_lengths, scale = params
+    lengths = tensors[-1] if has_lengths else None
+    return getattr(torch.ops.conductor, name)(*(tensors[:-1] if has_lengths else tensors), *numbers, lengths, scale)
+
+
 def _refuse_gradients(name, tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ExecutionError(f"{name}: an input requires grad but the operator has no backward; call it under "
@@ -177,19 +183,17 @@ def _build_prefix(q, has_lengths, scale):
 
 
 def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None, direct=False):
-    op = (lambda: torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)) if direct else None
     window, sinks, scale = operator.index(window), operator.index(sinks), None if scale is None else float(scale)
     if lengths is None:
-        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v), op)
-    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths), op)
+        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v), direct)
+    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths), direct)
 
 
 def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None, direct=False):
-    op = (lambda: torch.ops.conductor.prefix_attention(q, prefix_k, prefix_v, k, v, lengths, scale)) if direct else None
     scale = None if scale is None else float(scale)
     if lengths is None:
-        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v), op)
-    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths), op)
+        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v), direct)
+    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths), direct)
 
 
 # ---------------------------------------------------------------- graph form
