@@ -452,8 +452,10 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
           for (int i = 0; i < 4; ++i) o[j][e][i] = 0.0f;
     }
 
-    if (!sm100::mbar_wait(&bars[st], phase)) {
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[st], phase))) {       // the whole warp gives up, or none of it
       if (lane == 0) sm100::report_timeout(args.status, 60);
+      for (int k = 0; k < L::STAGES && u + k < u_end; ++k)                    // its copies in flight, as long again
+        sm100::mbar_wait(&bars[(st + k) % L::STAGES], phase ^ ((st + k) / L::STAGES));
       break;
     }
     float s[4][4];

@@ -76,7 +76,7 @@ struct TileSmem {
 
 enum { B_QFULL = 0, B_QEMPTY = 1, B_FULL = 2, B_EMPTY = B_FULL + KV_STAGES, B_SFULL = B_EMPTY + KV_STAGES, B_PFULL = B_SFULL + 2,
        B_PVDONE = B_PFULL + 2, B_OFREE = B_PVDONE + 2, B_TFULL = B_OFREE + 2, B_TEMPTY = B_TFULL + TILE_SLOTS,
-       B_COUNT = B_TEMPTY + TILE_SLOTS };
+       B_DRAIN = B_TEMPTY + TILE_SLOTS, B_COUNT };
 static_assert(B_COUNT * 8 + 8 + TILE_SLOTS * 8 <= 256, "barrier block");
 
 // One tile: its rows and its list of key blocks.  Entry j of the list is prefix block p0 + j for j < np, else
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      int ring = 0;
+      int ring = 0, loads = 0, q_loads = 0;
       bool ok = true;
       int idx = static_cast<int>(blockIdx.x);
       for (int k = 0; ok; ++k) {
@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         if (k > 0 && !sm100::mbar_wait(&bars[B_QEMPTY], (k - 1) & 1)) { sm100::report_timeout(t.status, 41); break; }
         const int q_bytes = PACKED ? a.Sq * a.G * t.seqs_per_half * HD * 2 : L::TILE_BYTES;
         sm100::mbar_arrive_expect_tx(&bars[B_QFULL], (r.live[0] + r.live[1]) * q_bytes);
+        q_loads = k + 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (r.live[h])
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
           const int n = ring + i, st = n % KV_STAGES, use = n / KV_STAGES, j = i >> 1;
           if (use > 0 && !sm100::mbar_wait(&bars[B_EMPTY + st], (use - 1) & 1)) { sm100::report_timeout(t.status, 42); ok = false; break; }
           sm100::mbar_arrive_expect_tx(&bars[B_FULL + st], L::TILE_BYTES);
+          loads = n + 1;
           const bool pre = PACKED || j < r.np;
           const void* tmap = pre ? ((i & 1) ? static_cast<const void*>(&t.tmap_pv) : static_cast<const void*>(&t.tmap_pk))
                                  : ((i & 1) ? static_cast<const void*>(&t.tmap_v) : static_cast<const void*>(&t.tmap_k));
@@ -288,6 +290,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
         }
         ring += 2 * r.n_iter;
       }
+      // no copy is in flight when the CTA ends, where a wait gave up either
+      for (int n = max(loads - KV_STAGES, 0); n < loads; ++n) sm100::mbar_wait(&bars[B_FULL + n % KV_STAGES], (n / KV_STAGES) & 1);
+      if (q_loads > 0) sm100::mbar_wait(&bars[B_QFULL], (q_loads - 1) & 1);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (convergent warp, elected lane)
@@ -423,6 +428,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       }
       ring += 2 * n_iter;
     }
+    if (!ok) {                    // products in flight end before their tensor memory is freed
+      commit(&bars[B_DRAIN]);
+      sm100::mbar_wait(&bars[B_DRAIN], 0);
+    }
   } else if (warp >= SOFTMAX_WARP0) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     // ------------------------------------------------------------ softmax / correction / epilogue
@@ -433,11 +442,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
     const uint32_t s_taddr = tmem_base + TMEM_S + g * 128 + lane_sel;
     const uint32_t o_taddr = tmem_base + TMEM_O + g * 128 + lane_sel;
     unsigned char* stage = smem + L::STAGE_OFF + (warp - SOFTMAX_WARP0) * L::WARP_STAGE;
+    bool ok = true;      // a wait that gives up does so for the whole warp: what its lanes do together would wait for one that left
     int n = 0;                                       // key blocks consumed so far over all tiles
-    bool ok = true;
     for (int k = 0; ok; ++k) {
       const int slot = k % TILE_SLOTS;
-      if (!sm100::mbar_wait(&bars[B_TFULL + slot], (k / TILE_SLOTS) & 1)) { sm100::report_timeout(t.status, 51); break; }
+      if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[B_TFULL + slot], (k / TILE_SLOTS) & 1))) { sm100::report_timeout(t.status, 51); break; }
       const int idx = tile_ring[2 * slot], len = tile_ring[2 * slot + 1];
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&bars[B_TEMPTY + slot]);
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 
       for (int j = 0; j < r.n_iter; ++j) {
         if (j >= pre && (j < wa || j > wb)) continue;
-        if (!sm100::mbar_wait(&bars[B_SFULL + g], n & 1)) { sm100::report_timeout(t.status, 52); ok = false; break; }
+        if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[B_SFULL + g], n & 1))) { sm100::report_timeout(t.status, 52); ok = false; break; }
         ++n;
         sm100::tc_fence_after();
         if (!PACKED && j == 0 && light) {
@@ -565,7 +574,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
       const bool none = !live || (!PACKED && pos < 0) || l == 0.0f;
       const float inv = 1.0f / l;
       if (live) {
-        if (!sm100::mbar_wait(&bars[B_PVDONE + g], (n - 1) & 1)) { sm100::report_timeout(t.status, 53); ok = false; break; }
+        if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars[B_PVDONE + g], (n - 1) & 1))) { sm100::report_timeout(t.status, 53); ok = false; break; }
         sm100::tc_fence_after();
       }
       if constexpr (PACKED) {
