@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(StreamSmem<HD>::THREADS, 1) stream_attention_k
       float v = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
                       fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
       v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-      mx[x] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)) * a.scale_log2;     // scale > 0: the maximum commutes with it
+      // scale > 0: the maximum commutes with it
+      mx[x] = fmaf(fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)), a.scale_log2, -WeightShift<BF16>::value);
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] + SA_RESCALE || mx[1] > m[1] + SA_RESCALE)) {
 #pragma unroll

@@ -64,6 +64,14 @@ struct StreamPlan {
   int64_t tasks, slots, units;     // units of 32 keys: the most there can be (every sequence at full length)
 };
 
+// The weights of a row are rounded to the input type for the second product (the matrix instructions take both operands in one
+// 16-bit type): relative 2^-8 at most each at bf16, 2^-11 at f16, independent from key to key.  f16 ends at 2^-24, and
+// against a dominating key the many weights of a long cache can all be smaller.  There the reference of the exponentials is
+// the running maximum minus 7: the largest weight is 2^7 (2^15 before a rescale, below the type's 2^16) and weights count down
+// to 2^-32.  Sums are taken against the same reference, so nothing else changes.
+template <bool BF16>
+struct WeightShift { static constexpr float value = BF16 ? 0.0f : 7.0f; };   // log2 units
+
 // Many query rows (cdr_tile_attention.cu).  Their `ws` is kTileCounterBytes for the tile counter, 32-byte aligned.
 constexpr size_t kTileCounterBytes = 256;
 // prefix, sinks and window of every (sequence, query head), 256 queries per tile

@@ -109,7 +109,7 @@ __device__ __forceinline__ void softmax_sinks(int see, float scale_log2, uint32_
     if (i >= see) sr[i] = __float_as_uint(-INFINITY);
     top = fmaxf(top, __uint_as_float(sr[i]));
   }
-  m_ref = top * scale_log2;
+  m_ref = fmaf(top, scale_log2, -WeightShift<BF16>::value);
   const float neg_m = m_ref == -INFINITY ? 0.0f : -m_ref;
   float sum = 0.0f;
 #pragma unroll
@@ -531,13 +531,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tile_attention_kernel(const __g
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               mx[i & 3] = max3(mx[i & 3], __uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1]));
-          m_ref = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          m_ref = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), a.scale_log2, -WeightShift<BF16>::value);
           const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
           store_p<BF16, 0, false>(sr, a.scale_log2, neg_m, l0, l1, s_taddr);
         } else {
           float l0s = l0, l1s = l1;
           const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
-          const float bmax = store_p<BF16, 0, true>(sr, a.scale_log2, neg_m, l0s, l1s, s_taddr) * a.scale_log2;
+          const float bmax = fmaf(store_p<BF16, 0, true>(sr, a.scale_log2, neg_m, l0s, l1s, s_taddr), a.scale_log2, -WeightShift<BF16>::value);
           if (__any_sync(0xffffffffu, bmax > m_ref + kRescale)) {
             const float m_new = fmaxf(m_ref, bmax);
             const float alpha = (m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);

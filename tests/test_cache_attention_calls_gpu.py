@@ -1,4 +1,5 @@
 """How window_attention and prefix_attention may be called: threads, transforms and tracers, views, single queries, repeats."""
+import math
 import os
 import subprocess
 import sys
@@ -13,7 +14,7 @@ import conductor
 from cache_attention_ref import check, reference
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.compiler.gcu_backend import get_gcu_backend
-from test_cache_attention_gpu import PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
+from test_cache_attention_gpu import DEV, PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 ROOT = Path(__file__).resolve().parent.parent
@@ -196,3 +197,29 @@ torch.save([t.cpu() for t in out], sys.argv[1])
         subprocess.run([sys.executable, "-c", code, str(path)], env={**os.environ, **extra}, check=True, timeout=300)
         got.append(torch.load(path))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("B,H,Sq,keys,P", [(1, 1, 1, 100000, 0), (1, 2, 3, 9000, 0), (40, 2, 1, 20000, 0), (2, 1, 300, 16000, 0), (40, 2, 1, 64, 16000)])
+def test_small_f16_weights_beside_a_dominating_key(B, H, Sq, keys, P):
+    """One key of weight 1 with value 0 and many of weight 2^-25.6, below what f16 holds, with value 1.
+
+    Scores are exact.  A weight w counts to within 2^-32 of the largest (half a step of the smallest f16, seven binary places down), the
+    output is rounded once (2^-11 relative, 2^-25 below the smallest normal); fp32 sums and exponentials: 2^-18."""
+    def near(*shape):
+        k = torch.zeros(*shape, 64, dtype=torch.float16, device=DEV)
+        v = torch.ones_like(k)
+        k[..., 0, 0], v[..., 0, :] = 17.75, 0.0
+        return k, v
+
+    q = torch.zeros(B, H, Sq, 64, dtype=torch.float16, device=DEV)
+    q[..., 0] = 8.0                                                 # score = the key's first element
+    weight = math.exp(-17.75)
+    if P:
+        k = torch.zeros(B, H, keys, 64, dtype=torch.float16, device=DEV)
+        got = PREFIX(q, *near(H, P), k, torch.ones_like(k))
+    else:
+        got = WINDOW(q, *near(B, H, keys), 1 << 30)
+    seen = torch.arange(keys - Sq, keys, device=DEV, dtype=torch.float64) + P      # keys of weight 2^-25.6 that row i sees
+    want = (seen * weight / (1 + seen * weight)).view(1, 1, Sq, 1)
+    bound = seen.view(1, 1, Sq, 1) * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -25
+    assert ((got.double() - want).abs() <= bound).all(), (got.flatten()[0].item(), want.flatten()[0].item())
