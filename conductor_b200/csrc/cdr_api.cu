@@ -333,11 +333,6 @@ int cdr_execute_host(int template_id, const cdr_tensor* host_inputs, int n_input
   if (device < 0 || device >= kMaxDevices) { set_error("device %d out of range", device); return CDR_ERR_BAD_ARG; }
   CDR_CUDA_TRY(cudaSetDevice(device));
 
-  size_t ws_bytes = 0;
-  if (int rc = cdr_workspace_bytes(template_id, host_inputs, n_inputs, host_outputs, n_outputs, params, params_bytes,
-                                   &ws_bytes))
-    return rc;
-
   std::vector<cdr_tensor> din, dout;
   std::vector<size_t> off;
   size_t total = 0;
@@ -349,6 +344,12 @@ int cdr_execute_host(int template_id, const cdr_tensor* host_inputs, int n_input
     set_error("out of host memory");
     return CDR_ERR_BAD_ARG;
   }
+  // the size of the scratch, asked for tensors that lie as they will on the device: host memory may have any alignment
+  for (cdr_tensor& t : din) t.data = reinterpret_cast<void*>(uintptr_t(256));
+  for (cdr_tensor& t : dout) t.data = reinterpret_cast<void*>(uintptr_t(256));
+  size_t ws_bytes = 0;
+  if (int rc = cdr_workspace_bytes(template_id, din.data(), n_inputs, dout.data(), n_outputs, params, params_bytes, &ws_bytes)) return rc;
+
   for (int i = 0; i < n_inputs; ++i) {
     if (!is_contiguous(din[i])) { set_error("host input %d is not contiguous", i); return CDR_ERR_BAD_ARG; }
     off.push_back(total);

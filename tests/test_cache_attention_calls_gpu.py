@@ -11,9 +11,12 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 import conductor
+from abi_util import execute_host
 from cache_attention_ref import check, reference
 from conductor.utils.exceptions import ExecutionError
 from conductor_b200.compiler.gcu_backend import get_gcu_backend
+from conductor_b200.codegen.kernel_templates import CdrWindowAttnParams
+from conductor_b200.codegen.operator_registry import Template
 from test_cache_attention_gpu import DEV, PREFIX, WINDOW, cache, lens, no_wait_gave_up, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -223,3 +226,14 @@ def test_small_f16_weights_beside_a_dominating_key(B, H, Sq, keys, P):
     want = (seen * weight / (1 + seen * weight)).view(1, 1, Sq, 1)
     bound = seen.view(1, 1, Sq, 1) * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -25
     assert ((got.double() - want).abs() <= bound).all(), (got.flatten()[0].item(), want.flatten()[0].item())
+
+
+def test_host_tensors_of_any_alignment():
+    """The host entry point stages its tensors: where they lie in host memory does not matter."""
+    q, k, v = cache(2, 4, 2, 3, 90, 64)
+    p = CdrWindowAttnParams(0.125, 0, 20, 2)
+    odd = [torch.empty(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    out = torch.empty(q.numel() + 1, dtype=q.dtype)[1:].view(q.shape)
+    assert all(t.data_ptr() % 16 for t in (*odd, out))
+    assert execute_host(Template.WINDOW_ATTENTION, odd, [out], p) == 0
+    check(out.to(DEV), reference(q, k, v, window=20, sinks=2))
