@@ -927,7 +927,8 @@ int parse_problem(const char* op, const cdr_tensor* ins, int n_in, const cdr_ten
   if (q.dtype != CDR_BF16 && q.dtype != CDR_F16) { set_error("%s: dtype %d unsupported (bf16 and f16 only)", op, q.dtype); return CDR_ERR_UNSUPPORTED; }
   const int64_t B = q.shape[0], Hq = q.shape[1], Sq = q.shape[2], D = q.shape[3];
   if (D != 64 && D != 128) { set_error("%s: head dim %lld unsupported (64 or 128)", op, (long long)D); return CDR_ERR_UNSUPPORTED; }
-  if (!(scale > 0.0f) || !isfinite(scale)) { set_error("%s: scale must be positive and finite", op); return CDR_ERR_UNSUPPORTED; }
+  // (in powers of two too, as the kernels use it: an infinite factor would turn scores of 0 into NaN)
+  if (!(scale > 0.0f) || !isfinite(scale * 1.4426950408889634f)) { set_error("%s: scale must be positive and finite", op); return CDR_ERR_UNSUPPORTED; }
   if (int rc = check_operand(q, op, "q", 4, q.dtype, D, &a->sq)) return rc;
   if (int rc = check_operand(k, op, "k", 4, q.dtype, D, &a->sk)) return rc;
   if (int rc = check_operand(v, op, "v", 4, q.dtype, D, &a->sv)) return rc;

@@ -160,3 +160,10 @@ def test_debug_artifacts_name_the_operators(tmp_path):
     path = DebugArtifactManager(str(tmp_path)).save_clusters("kernel", plan.launches)
     names = [row["template"] for row in json.loads(path.read_text())]
     assert "window_attention" in names and "prefix_attention" in names and not any(n.isdigit() for n in names)
+
+
+def test_scale_must_be_finite_in_powers_of_two(built_library):
+    q, k, v = cache()
+    for scale, status in ((2.3e38, 0), (2.4e38, -2), (float("nan"), -2), (1e-45, 0)):
+        assert _workspace(Template.WINDOW_ATTENTION, [q, k, v], torch.empty_like(q), kt.CdrWindowAttnParams(scale, 0, 4, 0))[0] == status
+        assert _workspace(Template.PREFIX_ATTENTION, [q, k[0], v[0], k, v], torch.empty_like(q), kt.CdrPrefixAttnParams(scale, 0))[0] == status
