@@ -24,8 +24,8 @@
 // the same call gives the same bits) and those of the shared prefix (cdr_tile_attention.cu).  Where there are
 // few tasks, a task belongs to one thread-block cluster instead, whose warps join their parts through
 // distributed shared memory: one launch, no scratch (one sequence: 11.2 -> 8.7 us).
-// P is rounded to the input type for the second product (relative 2^-8 at most per weight at bf16, independent per
-// key); scores, maxima, sums and O stay in fp32.
+// P is rounded to the input type for the second product (WeightShift in cdr_cache_attention.cuh says how far); scores, maxima,
+// sums and O stay in fp32.
 // Measured (B200): 64 sequences of up to 4096 keys, 32 / 8 heads, window 2048: 85 us, 5.5 TB/s of 465 MB with both
 // kernels; long caches (64 x 4096 keys, 2 x 131072) 6.2 TB/s, of 6.5 that a plain copy reaches.  Shorter calls are
 // bound by the latency of two dependent launches or of the cluster's exchange.
@@ -1029,6 +1029,11 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // 8 sequences, 32 / 8 heads, 4096 keys: 16 queries 97 streamed / 128 in tiles, 24 queries 144 / 128; 1 sequence: 48 queries
 // 49 / 63.  Prefix of 4096 keys, 8 heads, 64 own keys: 4 sequences 14 streamed / 18 packed, 8 sequences 24 / 18, 64 118 / 21;
 // of 16384: 2 sequences 24 / 29, 4 sequences 37 / 33.
+// The streaming estimate has no term for the memory's rate: one sequence of 131072 keys is put at 69 and takes 93.
+// From 256 queries on tiles are taken without an estimate, whose walk over all row tiles would cost a prompt's call more than its
+// launch.  That is right where the heads fill the machine and wrong where few of them stand before a long cache; 256 queries, us,
+// tiles / streamed: 8 sequences of 32 / 8 heads, 4096 keys 141 / 1751; 1 of 32 / 8, 8192 keys 131 / 408, window 512 21 / 112;
+// but 1 of 8 / 8, 4096 keys 68 / 61; 1 of 4 / 4, 32768 keys 496 / 184.
 CachePlan plan_call(const CacheAttn& a) {
   CachePlan c;
   c.packed_bytes = 0;

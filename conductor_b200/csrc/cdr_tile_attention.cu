@@ -22,9 +22,11 @@
 // What bounds it: the chain softmax -> own products -> softmax of a half, and the MMA warp, which in a build with clocks in
 // the kernel was busy for 2950 of the 3770 cycles of a block pair (32 products of 64.6 cycles, see cdr_attention.cu, are
 // 2067 of them; the rest are barriers, commits and hand-overs).  Measured
-// (B200): 4 x 1024 queries behind 4096 shared keys 167 us, 0.92 PFLOP/s of 1.60 that a large library product reaches; an
-// 8192 prompt with a window of 2048 269 us, 0.90; 8 x 2048 with a window of 512 118 us, 0.51 (masked halves of edge
-// blocks, and an epilogue every 5 blocks).
+// (B200, twelve calls at a time in a captured graph; a loop of calls under the power limit in brackets): 4 x 1024 queries behind
+// 4096 shared keys 166 us [180], 0.93 PFLOP/s [0.86] of 1.60 that a large library product reaches; an 8192 prompt with a
+// window of 2048 268 us [293], 0.90 [0.82]; 8 x 2048 with a window of 512 116 us [125], 0.52 [0.48] (masked halves of
+// edge blocks, and an epilogue every 5 blocks).
+// P is rounded to the input type for the second product, as in cdr_cache_attention.cu.
 // Measured and dropped: products cut to the visible keys in every edge block (operand shapes that the issuing warp computes
 // at run time: 172 -> 205 us on the first case).
 #include <cuda.h>

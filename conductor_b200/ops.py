@@ -17,7 +17,7 @@ dispatcher as ``torch.ops.conductor.*``.
 Common to both: ``q`` is ``[B, Hq, Sq, D]``, the cache ``[B, Hkv, Skv, D]``, ``Hq`` a multiple of ``Hkv``
 (query heads ``h*G .. h*G + G-1`` share key head ``h``); bf16 or f16; ``D`` 64 or 128.  Views are read in
 place when ``D`` is contiguous and the other strides are multiples of 8 elements, otherwise they are
-gathered first.  ``lengths`` (``[B]``, int32 or int64, on the same device) is how many keys each
+gathered first (and so are views made inside a compiled function).  ``lengths`` (``[B]``, int32 or int64, on the same device) is how many keys each
 sequence uses, clamped to ``0 .. Skv``; what the cache holds behind them does not matter.  Query ``i`` stands
 at position ``p = L - Sq + i``; a query with ``p < 0`` sees nothing, and a query that sees nothing
 returns 0.  ``scale`` defaults to ``1 / sqrt(D)`` and is positive (a constant inside compiled functions).  The result is contiguous ``[B, Hq, Sq, D]``.
