@@ -27,6 +27,7 @@ Among the keys in use, a non-finite value of ``k`` or ``v`` that some queries se
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 import threading
 from typing import Optional
@@ -57,7 +58,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         return torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)
     if q.__class__ is not torch.Tensor and has_torch_function_variadic(q):
         return torch.ops.conductor.window_attention(q, k, v, window, sinks, lengths, scale)
-    return _run_window(q, k, v, window, sinks, lengths, scale, True)
+    return _run_window(q, k, v, window, sinks, lengths, scale, _direct_run)
 
 
 def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -66,7 +67,7 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
     (``[Hkv, P, D]``, ``P >= 0``, the same for all sequences) and the keys ``j <= p`` of its own sequence."""
     if torch.compiler.is_compiling() or (q.__class__ is not torch.Tensor and has_torch_function_variadic(q)):
         return torch.ops.conductor.prefix_attention(q, prefix_k, prefix_v, k, v, lengths, scale)
-    return _run_prefix(q, prefix_k, prefix_v, k, v, lengths, scale, True)
+    return _run_prefix(q, prefix_k, prefix_v, k, v, lengths, scale, _direct_run)
 
 
 # ---------------------------------------------------------------- direct calls
@@ -111,7 +112,7 @@ class _Call:
         return out
 
 
-def _run(name, build, params, tensors, direct):
+def _run(name, build, params, tensors, other):
     try:
         call = _calls.last.get((name, params))
     except AttributeError:                         # this thread's first call
@@ -120,23 +121,29 @@ def _run(name, build, params, tensors, direct):
         out = call(tensors)
         if out is not None:
             return out
-    return _other_run(name, build, params, tensors, direct)
+    return other(name, build, params, tensors)
 
 
-def _other_run(name, build, params, tensors, direct):
-    """A call that is not the last one of its parameters again: found among the kept ones, or made; a direct call is left
-    to the dispatcher where something besides the kernel has to see it."""
-    if direct and has_torch_function([t for t in tensors if type(t) not in (torch.Tensor, torch.nn.Parameter)]):
+def _direct_run(name, build, params, tensors):
+    """A direct call that is not the last one of its parameters again; left to the dispatcher where something besides the
+    kernel has to see it."""
+    special = [t for t in tensors if type(t) not in (torch.Tensor, torch.nn.Parameter)]
+    if has_torch_function(special):
         return _dispatched(name, params, tensors)
-    if not all(isinstance(t, torch.Tensor) for t in tensors):
+    if not all(isinstance(t, torch.Tensor) for t in special):
         raise ExecutionError(f"{name}: expected tensors, got {[type(t).__name__ for t in tensors]}", kernel_name=name)
-    if direct and any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors):
+    if special:
         return _dispatched(name, params, tensors)
+    if tensors[0].device.type == "cuda" and load_call_module().is_dispatched(*tensors):
+        return _dispatched(name, params, tensors)
+    return _other_run(name, build, params, tensors)
+
+
+def _other_run(name, build, params, tensors):
+    """The kernel's call: found among the kept ones, or made."""
     device = tensors[0].device
     if device.type != "cuda":
         raise DeviceError(f"{name}: kernel templates run on CUDA tensors, got {device}")
-    if direct and load_call_module().is_dispatched(*tensors):
-        return _dispatched(name, params, tensors)
     for t in tensors:
         if t.device != device:
             raise ExecutionError(f"{name}: tensors on {device} and {t.device}", kernel_name=name)
@@ -157,6 +164,13 @@ def _other_run(name, build, params, tensors, direct):
             return get_executor().execute(launch, tensors)[0]
     _calls.last[(name, params)] = call
     return out
+
+
+def _autograd_run(name, build, params, tensors):
+    """The operators' autograd kernel where the kept call does not apply: there is no gradient to give."""
+    _refuse_gradients(name, tensors)
+    with torch._C._AutoDispatchBelowAutograd():
+        return _dispatched(name, params, tensors)
 
 
 def _dispatched(name, params, tensors):
@@ -182,18 +196,18 @@ def _build_prefix(q, has_lengths, scale):
     return prefix_attention_launch("prefix_attention", q.shape, q.dtype, has_lengths, scale)
 
 
-def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None, direct=False):
+def _run_window(q, k, v, window, sinks=0, lengths=None, scale=None, other=_other_run):
     window, sinks, scale = operator.index(window), operator.index(sinks), None if scale is None else float(scale)
     if lengths is None:
-        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v), direct)
-    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths), direct)
+        return _run("window_attention", _build_window, (window, sinks, False, scale), (q, k, v), other)
+    return _run("window_attention", _build_window, (window, sinks, True, scale), (q, k, v, lengths), other)
 
 
-def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None, direct=False):
+def _run_prefix(q, prefix_k, prefix_v, k, v, lengths=None, scale=None, other=_other_run):
     scale = None if scale is None else float(scale)
     if lengths is None:
-        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v), direct)
-    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths), direct)
+        return _run("prefix_attention", _build_prefix, (False, scale), (q, prefix_k, prefix_v, k, v), other)
+    return _run("prefix_attention", _build_prefix, (True, scale), (q, prefix_k, prefix_v, k, v, lengths), other)
 
 
 # ---------------------------------------------------------------- graph form
@@ -202,22 +216,8 @@ _lib.define("window_attention(Tensor q, Tensor k, Tensor v, int window, int sink
 _lib.define("prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? lengths=None, float? scale=None) -> Tensor")
 _lib.impl("window_attention", _run_window, "CUDA")
 _lib.impl("prefix_attention", _run_prefix, "CUDA")
-
-
-def _no_gradients(name):
-    """The autograd kernel of an operator without a gradient: refuses the call that needs one, else passes it on."""
-    op = getattr(torch.ops.conductor, name).default
-
-    def kernel(*args, **kwargs):
-        _refuse_gradients(name, [t for t in (*args, *kwargs.values()) if isinstance(t, torch.Tensor)])
-        with torch._C._AutoDispatchBelowAutograd():
-            return op(*args, **kwargs)
-
-    return kernel
-
-
-_lib.impl("window_attention", _no_gradients("window_attention"), "Autograd")
-_lib.impl("prefix_attention", _no_gradients("prefix_attention"), "Autograd")
+_lib.impl("window_attention", functools.partial(_run_window, other=_autograd_run), "Autograd")
+_lib.impl("prefix_attention", functools.partial(_run_prefix, other=_autograd_run), "Autograd")
 
 
 @torch.library.register_fake("conductor::window_attention", lib=_lib)
