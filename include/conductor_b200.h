@@ -236,8 +236,8 @@ typedef struct cdr_attn_params {
  * `lengths` ([B], i32 or i64, device memory like every input) is the number of keys each sequence uses,
  * L = clamp(lengths[b], 0, Skv) (Skv without it); k and v behind L are never used, whatever they hold.  Query i stands at
  * position p = L - Sq + i and sees key j when j <= p and (window attention) j > p - window or j < sinks.  A query with
- * p < 0 (a padded batch) sees nothing, and a query that sees nothing has output 0.  Non-finite values in the used
- * part of v may reach every query of the same head whose tile reads that key. */
+ * p < 0 (a padded batch) sees nothing, and a query that sees nothing has output 0.  With Sq = 1 keys that the query does
+ * not see are never used; with more queries, non-finite values of v that some of them see may reach others of the same head. */
 typedef struct cdr_window_attn_params {
   float scale;         /* softmax scale, positive and finite             */
   int32_t has_lengths; /* 1: lengths is the last input                   */
